@@ -26,6 +26,9 @@ extern "C" {
 
 /* ggml type codes of the weight formats (ggml/include/ggml.h GGML_TYPE_*). */
 enum { S3T_TYPE_F32 = 0, S3T_TYPE_F16 = 1, S3T_TYPE_Q8_0 = 8 };
+/* Element types of the operators that follow s3t_layernorm: F32, F16, BF16
+ * (ggml's code) and 8-bit e4m3 (no ggml code). */
+enum { S3T_TYPE_BF16 = 30, S3T_TYPE_E4M3 = 1000 };
 
 /* s3t_trunk_run flags: where the image and output buffers live. */
 enum {
@@ -250,6 +253,134 @@ int s3t_rope(int device, void *x, int groups, int L, int windowed, int bf16, voi
  * activation rounding of the output).  Device pointers. */
 int s3t_layernorm(int device, const float *x, int rows, const float *gamma, const float *beta, void *y16, int q8,
                   void *stream);
+
+/* --- 8-bit products and the operators around them ------------------------
+ * No counterpart in the reference, whose 8-bit path is Q8_0 weights on a CPU.
+ * s3t_quantize_fp8 makes 8-bit operands, s3t_gemm_fp8 multiplies them,
+ * s3t_norm_residual is the step between two blocks and can write the next
+ * product's operand, and s3t_rotary turns the heads that a product returned.
+ * Shared rules: device pointers on `device`, work enqueued on `stream` (a
+ * cudaStream_t, NULL: the default stream) in one kernel, no allocation and no
+ * workspace, so calls may overlap on several streams and be captured.  The
+ * first call of any entry point on a device prepares that device (allocates):
+ * make it before a capture.  The caller's current device is left as it was.
+ * Strides count elements.  Outputs overlap no input, except where in place is
+ * allowed below.  A call with no rows or tokens (or no columns) writes nothing
+ * and succeeds. */
+
+/* Rows of a matrix in device memory.  scale and scale_stride belong to e4m3
+ * matrices: the scale of column group g (128 columns; the last may be
+ * narrower) of row block i is scale[g * scale_stride + i].  A row block is one
+ * row of an activation and 128 rows of a weight; a value stands for its e4m3
+ * number times its block's scale.  e4m3 data is 16-byte aligned and its stride
+ * a multiple of 16; bytes between the columns and the stride are not read and
+ * not written. */
+typedef struct s3t_matrix {
+    void *data;
+    int64_t stride;
+    float *scale;
+    int64_t scale_stride;
+} s3t_matrix;
+
+/* x [rows][x_stride] (F32, F16 or BF16; `cols` columns) -> q: e4m3 values with
+ * a scale per 128 columns and block_rows rows (1: an activation, 128: a
+ * weight).  With a = max(largest magnitude of the block, 2^-100): scale =
+ * a / 448, value = e4m3(x * (448 / a)), every operation in fp32 to nearest
+ * even.  A block that holds an infinity or a NaN gets that as its scale and
+ * stands for NaN as a whole. */
+int s3t_quantize_fp8(int device, int type, const void *x_dev, int64_t rows, int64_t cols, int64_t x_stride,
+                     int block_rows, const s3t_matrix *q, void *stream);
+
+/* y[M][N] = act(x[M][K] * w[N][K]^T + bias) of an e4m3 activation x (row
+ * blocks of 1) and an e4m3 weight w (row blocks of 128): the products of a
+ * group of 128 columns are summed in fp32 and scaled by both scales, the
+ * groups are summed in fp32.  bias: [N] fp32 or NULL.  act: 0 none, 1 GELU-erf
+ * (as s3t_gemm_f16).  y_type: F32, F16, BF16, or E4M3, which quantizes the
+ * result as s3t_quantize_fp8 does with block_rows 1 (y->scale for [ceil(N /
+ * 128)][scale_stride >= M]), ready to be the next product's x.  Any M, N >= 0
+ * and K >= 1.  The result does not depend on what else runs.  A wait that runs
+ * out inside the kernel is reported by s3t_device_status. */
+int s3t_gemm_fp8(int device, const s3t_matrix *x, const s3t_matrix *w, const float *bias_dev, int M, int N, int K,
+                 int act, int y_type, const s3t_matrix *y, void *stream);
+
+/* The step between two transformer blocks, per row of `dim` columns:
+ *   h    = post-norm(y) with S3T_NORM_POST, else y
+ *   x'   = resid_scale * x + branch_scale * channel_scale * f(gate) * h
+ *   u    = pre-norm(x')
+ * Norms are RMSNorm, v / sqrt(mean(v^2) + eps) * weight + bias, or with
+ * S3T_NORM_LAYER LayerNorm, (v - mean) / sqrt(var + eps) * weight + bias.  f
+ * is the identity, or a sigmoid or tanh by flag.  Everything is computed in
+ * fp32; u is taken from x' before its rounding to resid_type. */
+enum {
+    S3T_NORM_LAYER = 1,
+    S3T_NORM_POST = 2,
+    S3T_NORM_GATE_SIGMOID = 4,
+    S3T_NORM_GATE_TANH = 8,
+};
+typedef struct s3t_norm_args {
+    int64_t rows;               /* [0, 2^31) */
+    int32_t dim;                /* [1, 16384] */
+    int32_t type;               /* of y and gate: F32, F16 or BF16 */
+    int32_t resid_type;         /* of x and x_out: F32 or `type` */
+    int32_t u_type;             /* of u: `type`, or E4M3 (quantized like s3t_quantize_fp8, block_rows 1) */
+    int32_t flags;
+    float eps;
+    float resid_scale;
+    float branch_scale;
+    const void *y;              /* the block's output, or NULL: x' = resid_scale * x */
+    int64_t y_stride;
+    const float *post_weight;   /* [dim] each, or NULL: 1 and 0 */
+    const float *post_bias;
+    const void *gate;           /* row r uses gate row r / gate_rows (gate_rows 1: one per token; the tokens of a
+                                 * sequence: one per sequence); NULL: 1 */
+    int64_t gate_stride;        /* 0: one gate row for all */
+    int64_t gate_rows;
+    const float *channel_scale; /* [dim], or NULL: 1 */
+    const void *x;              /* the residual */
+    int64_t x_stride;
+    void *x_out;                /* x' (may be x itself, with its stride), or NULL: not written */
+    int64_t x_out_stride;
+    const float *pre_weight;    /* [dim] each, or NULL: 1 and 0 */
+    const float *pre_bias;
+    s3t_matrix u;               /* the next block's input, or data NULL: no pre-norm */
+} s3t_norm_args;
+int s3t_norm_residual(int device, const s3t_norm_args *args, void *stream);
+
+/* Radians per position of each of the rot_dim / 2 pairs of rotary positions,
+ * freq[i] = base^(-2 i / rot_dim), and the magnitude to multiply by, scaled
+ * for contexts `factor` (>= 1) times the trained one:
+ *   LINEAR    freq / factor (position interpolation)
+ *   BASE      base * factor^(rot_dim / (rot_dim - 2))
+ *   BY_PARTS  pairs with more than `fast` full turns within original_len keep
+ *             their frequency, pairs with fewer than `slow` get freq / factor,
+ *             linear in the turns between; magnitude 0.1 ln(factor) + 1 (YaRN,
+ *             Peng et al. 2023)
+ * Host only: freq is host memory, to be copied to the device once. */
+enum { S3T_ROTARY_UNSCALED = 0, S3T_ROTARY_LINEAR = 1, S3T_ROTARY_BASE = 2, S3T_ROTARY_BY_PARTS = 3 };
+int s3t_rotary_frequencies(int rot_dim, double base, int scaling, double factor, double original_len, double fast,
+                           double slow, double *freq, float *magnitude);
+
+/* The heads of one tensor: token t, head h, column c is
+ * x[t * x_token_stride + h * x_head_stride + c], so token-major, head-major
+ * and packed projections (a pointer to the first head) are all views.  out may
+ * be x itself, with the same strides. */
+typedef struct s3t_rotary_view {
+    const void *x;
+    void *out;
+    int32_t heads;
+    int64_t x_token_stride, x_head_stride, out_token_stride, out_head_stride;
+} s3t_rotary_view;
+
+/* Turns the first rot_dim columns of every head of q and (unless NULL) k by
+ * positions[t] * freq[i]: pair i is columns (i, i + rot_dim / 2), or (2 i,
+ * 2 i + 1) with S3T_ROTARY_INTERLEAVED; S3T_ROTARY_INVERSE turns back (the
+ * magnitude still multiplies).  The other columns are copied.  The angle is
+ * exact to 2^-25 turns for positions up to 2^27.  The heads of a token whose
+ * position is negative (padding) are not written. */
+enum { S3T_ROTARY_INTERLEAVED = 1, S3T_ROTARY_INVERSE = 2 };
+int s3t_rotary(int device, const double *freq_dev, int rot_dim, float magnitude, const int64_t *positions_dev,
+               int64_t tokens, int type, int head_dim, const s3t_rotary_view *q, const s3t_rotary_view *k, int flags,
+               void *stream);
 
 /* No counterpart in the reference: failure-detection self-test.  One device
  * thread waits, for limit_ms (1..2000), on an mbarrier that nothing arrives

@@ -24,7 +24,11 @@ from typing import Sequence
 import numpy as np
 
 __all__ = ["GgufModel", "VisionTrunk", "VisionTrunkOutput", "MultiTrunk", "lib", "S3TError",
-           "IMAGES_ON_DEVICE", "OUTPUT_ON_DEVICE"]
+           "IMAGES_ON_DEVICE", "OUTPUT_ON_DEVICE",
+           "Matrix", "NormArgs", "RotaryView", "quantize_fp8", "gemm_fp8", "norm_residual", "rotary_frequencies",
+           "rotary", "TYPE_F32", "TYPE_F16", "TYPE_BF16", "TYPE_E4M3", "NORM_LAYER", "NORM_POST",
+           "NORM_GATE_SIGMOID", "NORM_GATE_TANH", "ROTARY_UNSCALED", "ROTARY_LINEAR", "ROTARY_BASE",
+           "ROTARY_BY_PARTS", "ROTARY_INTERLEAVED", "ROTARY_INVERSE"]
 
 _PKG = Path(__file__).resolve().parent
 LIB_PATH = _PKG / "libs3t.so"
@@ -34,6 +38,28 @@ IMAGE, DIM, GRID = 1008, 1024, 72
 
 class S3TError(RuntimeError):
     pass
+
+
+class Matrix(C.Structure):
+    """s3t_matrix: rows in device memory, `stride` elements apart, and for 8-bit matrices the scale of
+    column group g of row block i at scale[g * scale_stride + i]."""
+    _fields_ = [("data", C.c_void_p), ("stride", C.c_int64), ("scale", C.c_void_p), ("scale_stride", C.c_int64)]
+
+
+class NormArgs(C.Structure):
+    """s3t_norm_args: the step between two blocks (norm_residual)."""
+    _fields_ = [("rows", C.c_int64), ("dim", C.c_int32), ("type", C.c_int32), ("resid_type", C.c_int32),
+                ("u_type", C.c_int32), ("flags", C.c_int32), ("eps", C.c_float), ("resid_scale", C.c_float),
+                ("branch_scale", C.c_float), ("y", C.c_void_p), ("y_stride", C.c_int64), ("post_weight", C.c_void_p),
+                ("post_bias", C.c_void_p), ("gate", C.c_void_p), ("gate_stride", C.c_int64), ("gate_rows", C.c_int64),
+                ("channel_scale", C.c_void_p), ("x", C.c_void_p), ("x_stride", C.c_int64), ("x_out", C.c_void_p),
+                ("x_out_stride", C.c_int64), ("pre_weight", C.c_void_p), ("pre_bias", C.c_void_p), ("u", Matrix)]
+
+
+class RotaryView(C.Structure):
+    """s3t_rotary_view: the heads of one tensor, read at x and written at out (which may be x)."""
+    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("heads", C.c_int32), ("x_token_stride", C.c_int64),
+                ("x_head_stride", C.c_int64), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64)]
 
 
 _lib = None
@@ -66,6 +92,12 @@ def lib() -> C.CDLL:
         L.s3t_attention.argtypes = [i, p, p, p, i, i, i, i, p, p]
         L.s3t_rope.argtypes = [i, p, i, i, i, i, p]
         L.s3t_layernorm.argtypes = [i, p, i, p, p, p, i, p]
+        L.s3t_quantize_fp8.argtypes = [i, i, p, i64, i64, i64, i, C.POINTER(Matrix), p]
+        L.s3t_gemm_fp8.argtypes = [i, C.POINTER(Matrix), C.POINTER(Matrix), p, i, i, i, i, i, C.POINTER(Matrix), p]
+        L.s3t_norm_residual.argtypes = [i, C.POINTER(NormArgs), p]
+        L.s3t_rotary_frequencies.argtypes = [i, C.c_double, i, C.c_double, C.c_double, C.c_double, C.c_double,
+                                             C.POINTER(C.c_double), C.POINTER(C.c_float)]
+        L.s3t_rotary.argtypes = [i, p, i, C.c_float, p, i64, i, i, C.POINTER(RotaryView), C.POINTER(RotaryView), i, p]
         L.s3t_device_status.argtypes = [i]
         L.s3t_stem_noalloc.argtypes = [p, p, i, p, p]
         L.s3t_trunk_run_rgb8.argtypes = [p, p, i, i, i, p, i, p]
@@ -339,3 +371,48 @@ def preprocess_rgb8(device: int, rgb_ptr: int, width: int, height: int, batch: i
     the reference's bilinear_resize_rgb (tools/sam3_vision_trunk.cpp:33-66), bit-exact."""
     check(lib().s3t_preprocess_rgb8(device, C.c_void_p(rgb_ptr), width, height, batch, C.c_void_p(out_ptr),
                                     C.c_void_p(stream) if stream else None))
+
+
+TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_E4M3 = 0, 1, 30, 1000
+NORM_LAYER, NORM_POST, NORM_GATE_SIGMOID, NORM_GATE_TANH = 1, 2, 4, 8
+ROTARY_UNSCALED, ROTARY_LINEAR, ROTARY_BASE, ROTARY_BY_PARTS = 0, 1, 2, 3
+ROTARY_INTERLEAVED, ROTARY_INVERSE = 1, 2
+
+
+def quantize_fp8(device: int, type: int, x_ptr: int, rows: int, cols: int, x_stride: int, block_rows: int, q: Matrix,
+                 stream: int = 0) -> None:
+    """Device rows of `type` (TYPE_F32, TYPE_F16 or TYPE_BF16) -> the e4m3 matrix `q` with a scale per 128 columns
+    and `block_rows` rows (1: an activation, 128: a weight): s3t_quantize_fp8."""
+    check(lib().s3t_quantize_fp8(device, type, x_ptr, rows, cols, x_stride, block_rows, q, stream))
+
+
+def gemm_fp8(device: int, x: Matrix, w: Matrix, bias_ptr: int | None, m: int, n: int, k: int, act: int, y_type: int,
+             y: Matrix, stream: int = 0) -> None:
+    """y [m][n] = act(x [m][k] w [n][k]^T + bias) of e4m3 matrices with block scales (x per row, w per 128 rows);
+    act 1 is GELU; y_type TYPE_F32, TYPE_F16, TYPE_BF16, or TYPE_E4M3 for the next product's x: s3t_gemm_fp8."""
+    check(lib().s3t_gemm_fp8(device, x, w, bias_ptr, m, n, k, act, y_type, y, stream))
+
+
+def norm_residual(device: int, args: NormArgs, stream: int = 0) -> None:
+    """The step between two blocks: post-norm of a block's output, gate, scales and residual sum, and the next
+    block's pre-norm, in one pass: s3t_norm_residual."""
+    check(lib().s3t_norm_residual(device, args, stream))
+
+
+def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: int = ROTARY_UNSCALED, factor: float = 1.0,
+                       original_len: float = 0.0, fast: float = 32.0, slow: float = 1.0) -> tuple[np.ndarray, float]:
+    """(radians per position of each pair as float64, magnitude) of rotary positions, scaled for a context `factor`
+    times `original_len`: s3t_rotary_frequencies.  Host only."""
+    freq = np.empty(max(rot_dim // 2, 1), np.float64)
+    magnitude = C.c_float()
+    check(lib().s3t_rotary_frequencies(rot_dim, base, scaling, factor, original_len, fast, slow,
+                                       freq.ctypes.data_as(C.POINTER(C.c_double)), C.byref(magnitude)))
+    return freq, magnitude.value
+
+
+def rotary(device: int, freq_ptr: int, rot_dim: int, magnitude: float, positions_ptr: int, tokens: int, type: int,
+           head_dim: int, q: RotaryView, k: RotaryView | None = None, flags: int = 0, stream: int = 0) -> None:
+    """Turns the first rot_dim columns of the heads of q and k by position times frequency (device float64
+    frequencies, int64 positions; a negative position leaves its token unwritten): s3t_rotary."""
+    check(lib().s3t_rotary(device, freq_ptr, rot_dim, magnitude, positions_ptr, tokens, type, head_dim, q, k, flags,
+                           stream))

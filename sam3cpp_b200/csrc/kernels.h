@@ -185,6 +185,110 @@ struct MhaArgs {
 cudaError_t launch_mha32(const MhaArgs& a, cudaStream_t stream);
 cudaError_t mha32_prepare();
 
+// Element types of the operators below (the S3T_TYPE_* codes they stand for
+// are mapped by element_kind).
+enum ElementKind : int { kF32 = 0, kF16 = 1, kBF16 = 2, kE4M3 = 3 };
+
+// Columns of a scale group, and rows of a weight's scale block.
+constexpr int kScaleBlock = 128;
+
+// 8-bit block quantization: per 128 columns of a row (block_rows 1) or per
+// 128 x 128 block (block_rows 128), scale = amax / 448 and q = e4m3(x * 448 / amax).
+struct QuantizeArgs {
+    const void* x;            // [rows][x_stride] of `kind`
+    int64_t rows, cols, x_stride;
+    int kind;                 // ElementKind of x
+    int block_rows;           // 1 or 128
+    int vec;                  // rows of x are 16-byte aligned
+    uint8_t* q;               // [rows][q_stride] e4m3
+    int64_t q_stride;
+    float* scale;             // [ceil(cols/128)][scale_stride], one per row block
+    int64_t scale_stride;
+};
+cudaError_t launch_quantize_fp8(const QuantizeArgs& a, cudaStream_t stream);
+
+// y = act(sum_g xs[g][m] ws[g][n/128] sum_{k in group g} x[m][k] w[n][k] + bias[n])
+struct GemmFp8Args {
+    int M, N, K;
+    const uint8_t* x;         // [M][x_stride] e4m3
+    int64_t x_stride;
+    const float* xs;          // [ceil(K/128)][xs_stride >= M]
+    int64_t xs_stride;
+    const uint8_t* w;         // [N][w_stride] e4m3
+    int64_t w_stride;
+    const float* ws;          // [ceil(K/128)][ws_stride >= ceil(N/128)]
+    int64_t ws_stride;
+    const float* bias;        // [N] or null
+    int gelu;
+    int out;                  // ElementKind of y
+    void* y;                  // [M][y_stride]
+    int64_t y_stride;
+    float* ys;                // kE4M3: [ceil(N/128)][ys_stride >= M]
+    int64_t ys_stride;
+    int vec;                  // rows of y are 16-byte aligned
+    int* status;
+};
+cudaError_t launch_gemm_fp8(const GemmFp8Args& a, int num_sms, cudaStream_t stream);
+cudaError_t fp8_prepare();
+
+// The step between two blocks: h = post-norm(y) (or y), x' = resid_scale x +
+// branch_scale channel act(gate) h, u = pre-norm(x').
+enum GateAct : int { kGatePlain = 0, kGateSigmoid = 1, kGateTanh = 2 };
+struct NormResidualArgs {
+    int64_t rows;             // below 2^31
+    int dim;
+    int kind;                 // ElementKind of y, gate and (unless 8-bit) u
+    int resid_kind;           // ElementKind of x and x_out: kF32 or `kind`
+    int u_eight;              // u is e4m3 with scales
+    int layer;                // LayerNorm (1) or RMSNorm (0)
+    int post;                 // normalize y
+    int gate_act;             // GateAct
+    float eps, resid_scale, branch_scale;
+    const void* y;            // [rows][y_stride], or null: no branch
+    int64_t y_stride;
+    const float* post_weight; // [dim] each, or null: 1 and 0
+    const float* post_bias;
+    const void* gate;         // [ceil(rows / gate_rows)][gate_stride], or null: 1
+    int64_t gate_stride;
+    int gate_rows;
+    const float* channel;     // [dim], or null: 1
+    const void* x;            // [rows][x_stride]
+    int64_t x_stride;
+    void* x_out;              // [rows][x_out_stride], or null
+    int64_t x_out_stride;
+    const float* pre_weight;
+    const float* pre_bias;
+    void* u;                  // [rows][u_stride], or null: no pre-norm
+    int64_t u_stride;
+    float* u_scale;           // u_eight: [ceil(dim/128)][u_scale_stride]
+    int64_t u_scale_stride;
+    int vec;                  // every row starts at a 16-byte boundary
+};
+constexpr int kNormMaxDim = 16384;
+cudaError_t launch_norm_residual(const NormResidualArgs& a, cudaStream_t stream);
+
+// Rotary positions on the heads of one or two tensors of the same tokens.
+struct RotaryPart {
+    const void* x;            // token t, head h, column c at x[t * x_token + h * x_head + c]
+    void* out;
+    int heads;
+    int64_t x_token, x_head, out_token, out_head;
+};
+struct RotaryArgs {
+    const double* freq;       // [rot / 2] radians per position
+    int rot;                  // leading columns of a head that turn
+    float magnitude;
+    const int64_t* positions; // [tokens]; negative: the token's rows are not written
+    int64_t tokens;
+    int kind;                 // ElementKind: kF32, kF16 or kBF16
+    int head_dim;
+    int interleaved, inverse;
+    int vec;                  // 16-byte aligned heads, whole vectors on both sides of `rot`
+    RotaryPart part[2];       // part[1].heads may be 0
+};
+constexpr int kRotaryMaxDim = 1024;
+cudaError_t launch_rotary(const RotaryArgs& a, cudaStream_t stream);
+
 // Stem weights of a finalized context, for entry points defined outside
 // runtime.cu.  Returns false if the context is null or not finalized.
 struct StemView {
@@ -202,6 +306,10 @@ struct StemView {
 bool make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int elem_bytes, uint64_t inner,
                   uint64_t outer, uint32_t box_inner, uint32_t box_outer,
                   CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
+// Rows `stride_bytes` apart (a multiple of 16).
+bool make_tmap_rows(CUtensorMap* map, const void* base, CUtensorMapDataType dt, uint64_t inner, uint64_t outer,
+                    uint64_t stride_bytes, uint32_t box_inner, uint32_t box_outer,
+                    CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
 bool make_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int elem_bytes, uint64_t d0,
                   uint64_t d1, uint64_t d2, uint32_t b0, uint32_t b1,
                   CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
@@ -213,6 +321,28 @@ namespace s3t {
 bool ctx_stem_view(const s3t_ctx* ctx, StemView* out);
 // The context's own stream (what a NULL stream argument means), or null.
 cudaStream_t ctx_stream(const s3t_ctx* ctx);
+// What an op-level entry point outside runtime.cu needs of a device; prepares
+// the device on its first use.  Returns -1 with the message recorded on error.
+struct DeviceView {
+    int num_sms;
+    int* status;
+};
+int device_view(int device, DeviceView* out);
+// Makes `device` current and puts the caller's device back.
+struct DeviceScope {
+    int prev = -1;
+    cudaError_t error;
+    explicit DeviceScope(int device) {
+        error = cudaGetDevice(&prev);
+        if (error == cudaSuccess && prev != device) error = cudaSetDevice(device);
+        else if (error == cudaSuccess) prev = -1;
+    }
+    ~DeviceScope() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+    DeviceScope(const DeviceScope&) = delete;
+    DeviceScope& operator=(const DeviceScope&) = delete;
+};
 // Records the thread-local message returned by s3t_last_error(); returns -1.
 int set_last_error(const char* msg);
 }  // namespace s3t

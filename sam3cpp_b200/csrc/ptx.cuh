@@ -169,6 +169,22 @@ S3T_DEV void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+S3T_DEV uint32_t cluster_nctarank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+
+// Four floats of a CTA of the cluster by their shared::cluster address.
+S3T_DEV float4 ld_cluster_f4(uint32_t cluster_addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(cluster_addr)
+                 : "memory");
+    return v;
+}
+
 // Arrive on an mbarrier given by its shared::cluster address (possibly the
 // peer's), with the default release-at-CTA-scope semantics: enough to order
 // this warp's completed TMEM reads (tcgen05.fence::before_thread_sync) before
@@ -269,6 +285,16 @@ S3T_DEV void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint
         : "memory");
 }
 
+// As umma_f16_ss with kind::f8f6f4: 8-bit operands, 32 K elements per instruction.
+S3T_DEV void umma_f8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 // Arrive (once) on an mbarrier when all previously issued UMMAs of this thread complete.
 S3T_DEV void umma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
@@ -301,6 +327,15 @@ S3T_DEV void umma_f16_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
         : "memory");
 }
 
+S3T_DEV void umma_f8_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 // Arrive once on the mbarrier at this offset in every CTA of `cta_mask` when
 // the leader's previously issued pair MMAs complete.
 S3T_DEV void umma_commit_pair(uint64_t* bar, uint16_t cta_mask) {
@@ -321,6 +356,11 @@ __host__ __device__ constexpr uint32_t umma_idesc_f16(int M, int N, int ab_fmt, 
            | (uint32_t(b_mn_major) << 16)         // B major
            | (uint32_t(N >> 3) << 17)             // N / 8
            | (uint32_t(M >> 4) << 24);            // M / 16
+}
+
+// Instruction descriptor, kind::f8f6f4: D=f32, A and B e4m3 (format 0), both K-major, shape M x N.
+__host__ __device__ constexpr uint32_t umma_idesc_e4m3(int M, int N) {
+    return (1u << 4) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
 }
 
 // Shared-memory matrix descriptor, 128-byte swizzle (tile base 1024-aligned).

@@ -113,6 +113,7 @@ int device_state(int device, DeviceState** out) {
         S3T_CUDA(attention_prepare());
         S3T_CUDA(mha32_prepare());
         S3T_CUDA(neck_prepare());
+        S3T_CUDA(fp8_prepare());
         const std::vector<float> rl = rope_table(1.0f, kWindow);
         const std::vector<float> rg = rope_table(float(kWindow) / float(kGrid), kGrid);
         S3T_CUDA(cudaMalloc(&d.rope_local, rl.size() * 4));
@@ -867,6 +868,17 @@ int prepare_neck(s3t_ctx* c) {
 }  // namespace
 
 int s3t::set_last_error(const char* msg) { return fail(msg); }
+
+int s3t::device_view(int device, DeviceView* out) {
+    // device_state leaves the device it prepares current; the caller's comes back.
+    const DeviceScope scope(device);
+    if (scope.error != cudaSuccess) return fail(std::string("cudaSetDevice: ") + cudaGetErrorString(scope.error));
+    DeviceState* ds = nullptr;
+    if (device_state(device, &ds)) return -1;
+    out->num_sms = ds->num_sms;
+    out->status = ds->status;
+    return 0;
+}
 
 cudaStream_t s3t::ctx_stream(const s3t_ctx* c) { return c ? c->stream : nullptr; }
 
