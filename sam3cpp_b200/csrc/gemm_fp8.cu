@@ -47,14 +47,18 @@ S3T_DEV float2 packed_fma(float a0, float a1, float2 s, float2 c) { return __ffm
 
 template <int BN>
 struct TileCfg {
-    static constexpr int STAGES = BN == 16 ? 6 : BN == 32 ? 5 : BN == 64 ? 4 : 3;
+    static constexpr int STAGES = BN <= 32 ? 5 : BN == 64 ? 4 : 3;
     static constexpr int ACCS = BN == 128 ? 2 : 4;             // accumulators in flight
     static constexpr uint32_t TMEM_COLS = ACCS * BN;
     static constexpr uint32_t X_BYTES = BN * kStageRow;
     static constexpr uint32_t STAGE_BYTES = kHalfBytes + X_BYTES;
     static constexpr uint32_t RING = STAGES * STAGE_BYTES;
     static constexpr uint32_t RED_BYTES = BN * kTileM * 4;     // the fp32 tile, over the drained ring
-    static constexpr uint32_t SCALE_BYTES = 4 * 2 * BN * 4;    // [promotion warp][parity][column]
+    // Per promotion warp: a ring of raw scales (the block's and a row's per lane)
+    // and two buffers of their products.
+    static constexpr int SCALE_SLOTS = 4;
+    static constexpr int SCALE_WORDS = SCALE_SLOTS * 32 * ((BN + 31) / 32 + 1) + 2 * BN;
+    static constexpr uint32_t SCALE_BYTES = 4 * SCALE_WORDS * 4;
     static constexpr size_t SMEM = RING + SCALE_BYTES + 1024 + 256;
     static constexpr int THREADS = 192;
     static_assert(RED_BYTES <= RING, "the fp32 tile replaces the ring");
@@ -174,31 +178,39 @@ __global__ void __launch_bounds__(192)
     } else {
         // Promotion warp w: TMEM lanes (rows of w) 32 * (w % 4) .. + 31, all BN columns (rows of x).
         const int quarter = warp & 3;
-        float* my_scales = scales + (warp - 2) * 2 * BN;
         constexpr int PER_LANE = (BN + 31) / 32;
-        float next[PER_LANE];
+        // The scales of the BN rows and of the weight block come by cp.async,
+        // SCALE_SLOTS - 1 groups ahead, into words that only this lane reads: a
+        // load into a register would stall the warp at its first use.
+        float* raw = scales + (warp - 2) * Cfg::SCALE_WORDS + lane;
+        float* products = scales + (warp - 2) * Cfg::SCALE_WORDS + Cfg::SCALE_SLOTS * 32 * (PER_LANE + 1);
         const int nb = n0 / kScaleBlock;
         auto fetch = [&](int g) {
-            const float sw = __ldg(args.ws + int64_t(g) * args.ws_stride + nb);
+            float* slot = raw + ((g - g0) % Cfg::SCALE_SLOTS) * 32 * (PER_LANE + 1);
+            cp_async4(slot, g < g1 ? args.ws + int64_t(g) * args.ws_stride + nb : args.ws, g < g1);
 #pragma unroll
             for (int i = 0; i < PER_LANE; ++i) {
                 const int j = lane + 32 * i, m = m0 + j;
-                next[i] = j < BN && m < args.M ? __ldg(args.xs + int64_t(g) * args.xs_stride + m) * sw : 0.f;
+                const bool take = g < g1 && j < BN && m < args.M;
+                cp_async4(slot + 32 * (i + 1), take ? args.xs + int64_t(g) * args.xs_stride + m : args.xs, take);
             }
+            cp_async_commit();
         };
-        fetch(g0);
+        for (int i = 0; i < Cfg::SCALE_SLOTS - 1; ++i) fetch(g0 + i);
         float2 sum[BN / 2];
 #pragma unroll
         for (int i = 0; i < BN / 2; ++i) sum[i] = make_float2(0.f, 0.f);
         for (int i = 0; i < g1 - g0; ++i) {
             const int acc = i % Cfg::ACCS;
             const uint32_t aph = (i / Cfg::ACCS) & 1;
-            float* sc = my_scales + (i & 1) * BN;
+            fetch(g0 + i + Cfg::SCALE_SLOTS - 1);
+            cp_async_wait<Cfg::SCALE_SLOTS - 1>();
+            const float* slot = raw + (i % Cfg::SCALE_SLOTS) * 32 * (PER_LANE + 1);
+            float* sc = products + (i & 1) * BN;
 #pragma unroll
             for (int q = 0; q < PER_LANE; ++q)
-                if (lane + 32 * q < BN) sc[lane + 32 * q] = next[q];
+                if (lane + 32 * q < BN) sc[lane + 32 * q] = slot[32 * (q + 1)] * slot[0];
             __syncwarp();
-            if (i + 1 < g1 - g0) fetch(g0 + i + 1);
             if (!mbar_wait(tfull + acc, aph, args.status, kErrTimeoutEpilogue, abort_flag)) break;
             tc_fence_after();
             const uint32_t t = tmem_base + (uint32_t(quarter * 32) << 16) + acc * BN;
@@ -322,12 +334,404 @@ cudaError_t launch_tile(const GemmFp8Args& a, int num_sms, cudaStream_t stream) 
     return cudaLaunchKernelEx(&cfg, gemm_fp8_tile_kernel<BN, OUT>, tw, tx, a);
 }
 
+// -------------------------------------------------------------- many rows ---
+
+struct PairCfg8 {
+    static constexpr int BN = 256;
+    static constexpr int STAGES = 5;
+    static constexpr int WARPS = 8;                            // promotion and epilogue
+    static constexpr int WARP_COLS = BN * 4 / WARPS;           // 128: one weight block
+    static constexpr uint32_t STAGE_BYTES = 2 * kHalfBytes;    // 128 rows of x, 128 rows of w per CTA
+    static constexpr uint32_t RING = STAGES * STAGE_BYTES;
+    static constexpr uint32_t OUT_ROW = 64;                    // bytes of a row of y staged at a time
+    static constexpr uint32_t OUT_BUF = 32 * OUT_ROW;
+    static constexpr int OUT_BUFS = 3;                         // per warp
+    static constexpr uint32_t OUT_BYTES = WARPS * OUT_BUFS * OUT_BUF;
+    static constexpr int RAW_SLOTS = 6;                        // groups of scales on their way
+    static constexpr int RAW_WORDS = 64 * 4;                   // two row and two block scales per factor thread
+    static constexpr int FACTOR_SLOTS = 4;
+    static constexpr int FACTOR_WORDS = 2 * kTileM;            // a factor per row and weight block
+    static constexpr uint32_t SMALL_BYTES = 4 * (RAW_SLOTS * RAW_WORDS + FACTOR_SLOTS * FACTOR_WORDS + WARPS * WARP_COLS);
+    static constexpr uint32_t TMEM_COLS = 2 * BN;
+    static constexpr size_t SMEM = RING + OUT_BYTES + SMALL_BYTES + 1024 + 256;
+    // Warpgroup 0: TMA producer, UMMA issuer and two factor warps; warpgroups 1
+    // and 2: promotion.  The launch gives each of the 384 threads 168 registers
+    // (64,512 in all); 128 sums and the columns in flight need more, so
+    // warpgroup 0 keeps 40 (5,120) and the others take 224 (57,344).
+    static constexpr int THREADS = 128 + 32 * WARPS;
+    static constexpr int FEW_REGS = 40, MANY_REGS = 224;
+    static_assert(128 * FEW_REGS + 32 * WARPS * MANY_REGS <= THREADS * 168, "the split stays within the launch");
+};
+static_assert(PairCfg8::WARP_COLS == kScaleBlock, "a warp's columns lie in one weight block");
+
+template <int OUT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1)
+    gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                         const __grid_constant__ CUtensorMap tmY, const GemmFp8Args args) {
+    using Cfg = PairCfg8;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sX = smem;
+    uint8_t* sW = smem + Cfg::STAGES * kHalfBytes;
+    uint8_t* sOut = smem + Cfg::RING;
+    float* raw = reinterpret_cast<float*>(sOut + Cfg::OUT_BYTES);
+    float* factors = raw + Cfg::RAW_SLOTS * Cfg::RAW_WORDS;
+    float* biases = factors + Cfg::FACTOR_SLOTS * Cfg::FACTOR_WORDS;
+    uint64_t* full = reinterpret_cast<uint64_t*>(biases + Cfg::WARPS * Cfg::WARP_COLS);
+    uint64_t* empty = full + Cfg::STAGES;
+    uint64_t* tfull = empty + Cfg::STAGES;
+    uint64_t* tempty = tfull + 2;
+    uint64_t* drain = tempty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const int tiles_n = (args.N + Cfg::BN - 1) / Cfg::BN;
+    const int n_tiles = ((args.M + 2 * kTileM - 1) / (2 * kTileM)) * tiles_n;
+    const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+    const int groups = (args.K + kScaleBlock - 1) / kScaleBlock;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < Cfg::STAGES; ++s) {
+            mbar_init(full + s, 1);
+            mbar_init(empty + s, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(tfull + i, 1 + 2);             // the UMMAs and this CTA's factor warps
+            mbar_init(tempty + i, 2 * Cfg::WARPS);   // every promotion warp of the pair
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, Cfg::TMEM_COLS);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    cluster_sync();   // both CTAs' barriers exist before any cross-CTA arrive
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp < 4) {
+    setmaxnreg_dec<Cfg::FEW_REGS>();
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0, armed = 0, armed_parity = 0;
+            bool ok = true;
+            for (int tile = pair; ok && tile < n_tiles; tile += n_pairs) {
+                const int m0 = (tile / tiles_n) * 2 * kTileM + int(rank) * kTileM;
+                const int n0 = (tile % tiles_n) * Cfg::BN + int(rank) * kTileM;
+                for (int g = 0; g < groups; ++g) {
+                    if (!mbar_wait(empty + s, ph ^ 1, args.status, kErrTimeoutProducer, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t lfull = mapa_shared(smem_u32(full + s), 0);
+                    if (leader) {
+                        mbar_arrive_expect_tx(full + s, 2 * Cfg::STAGE_BYTES);
+                        armed |= 1u << s;
+                        armed_parity = (armed_parity & ~(1u << s)) | (ph << s);
+                    }
+                    tma_load_2d_pair(sX + s * kHalfBytes, &tmX, lfull, g * kScaleBlock, m0);
+                    tma_load_2d_pair(sW + s * kHalfBytes, &tmW, lfull, g * kScaleBlock, n0);
+                    if (++s == Cfg::STAGES) {
+                        s = 0;
+                        ph ^= 1;
+                    }
+                }
+            }
+            if (!ok && leader) {
+                // Gave up: wait (bounded) for the pair's copies counted on these barriers.
+                for (int i = 0; i < Cfg::STAGES; ++i)
+                    if (armed & (1u << i))
+                        mbar_wait(full + i, (armed_parity >> i) & 1u, args.status, kErrTimeoutDrain, nullptr);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            constexpr uint32_t idesc = umma_idesc_e4m3(2 * kTileM, Cfg::BN);
+            const uint64_t dX0 = umma_desc_sw128(smem_u32(sX), 16, 1024);
+            const uint64_t dW0 = umma_desc_sw128(smem_u32(sW), 16, 1024);
+            int s = 0, it = 0;
+            uint32_t ph = 0;
+            bool ok = true, issued = false;
+            for (int tile = pair; ok && tile < n_tiles; tile += n_pairs) {
+                for (int g = 0; g < groups; ++g, ++it) {
+                    const int acc = it & 1;
+                    const uint32_t aph = (it >> 1) & 1;
+                    if (!mbar_wait(tempty + acc, aph ^ 1, args.status, kErrTimeoutMma, abort_flag) ||
+                        !mbar_wait(full + s, ph, args.status, kErrTimeoutMma, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t dx = dX0 + uint64_t(s) * (kHalfBytes >> 4), dw = dW0 + uint64_t(s) * (kHalfBytes >> 4);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        umma_f8_ss_pair(tmem_base + acc * Cfg::BN, dx + 2 * k, dw + 2 * k, idesc, k != 0);
+                    issued = true;
+                    umma_commit_pair(empty + s, 0x3);
+                    umma_commit_pair(tfull + acc, 0x3);
+                    if (++s == Cfg::STAGES) {
+                        s = 0;
+                        ph ^= 1;
+                    }
+                }
+            }
+            if (!ok && issued) {
+                umma_commit_pair(drain, 0x1);
+                mbar_wait(drain, 0, args.status, kErrTimeoutDrain, nullptr);
+            }
+        }
+    } else {
+        // Factor warps: xs ws of this CTA's 128 rows and two weight blocks, for
+        // each group, so that a promotion warp reads one word.  The raw scales
+        // come by cp.async, RAW_SLOTS - 1 groups ahead, into words of the
+        // thread's own.  tfull of a group counts these warps too.
+        const int ft = int(threadIdx.x) - 64;
+        float* mine = raw + ft * 4;
+        int ahead_tile = pair - n_pairs, ahead_left = 0, ahead_slot = 0;
+        const float *x0 = args.xs, *x1 = args.xs, *w0 = args.ws, *w1 = args.ws;
+        bool in_x0 = false, in_x1 = false, in_w0 = false, in_w1 = false;
+        auto fetch = [&]() {
+            if (ahead_left == 0) {
+                ahead_tile += n_pairs;
+                const bool tile_ok = ahead_tile < n_tiles;
+                const int m = tile_ok ? (ahead_tile / tiles_n) * 2 * kTileM + int(rank) * kTileM + ft : 0;
+                const int n = tile_ok ? (ahead_tile % tiles_n) * Cfg::BN : 0;
+                in_x0 = tile_ok && m < args.M;
+                in_x1 = tile_ok && m + 64 < args.M;
+                in_w0 = tile_ok;
+                in_w1 = tile_ok && n + kScaleBlock < args.N;
+                x0 = args.xs + (in_x0 ? m : 0);
+                x1 = args.xs + (in_x1 ? m + 64 : 0);
+                w0 = args.ws + n / kScaleBlock;
+                w1 = in_w1 ? w0 + 1 : w0;
+                ahead_left = groups;
+            }
+            float* to = mine + ahead_slot * Cfg::RAW_WORDS;
+            cp_async4(to, x0, in_x0);
+            cp_async4(to + 1, x1, in_x1);
+            cp_async4(to + 2, w0, in_w0);
+            cp_async4(to + 3, w1, in_w1);
+            cp_async_commit();
+            ahead_slot = ahead_slot + 1 == Cfg::RAW_SLOTS ? 0 : ahead_slot + 1;
+            if (--ahead_left > 0) {   // the pointers stop at a tile's last group
+                x0 += args.xs_stride;
+                x1 += args.xs_stride;
+                w0 += args.ws_stride;
+                w1 += args.ws_stride;
+            }
+        };
+        for (int i = 0; i < Cfg::RAW_SLOTS - 1; ++i) fetch();
+        int it = 0, slot = 0;
+        bool ok = true;
+        for (int tile = pair; ok && tile < n_tiles; tile += n_pairs) {
+            for (int g = 0; g < groups; ++g, ++it) {
+                fetch();
+                cp_async_wait<Cfg::RAW_SLOTS - 1>();
+                const float4 s = *reinterpret_cast<const float4*>(mine + slot * Cfg::RAW_WORDS);
+                slot = slot + 1 == Cfg::RAW_SLOTS ? 0 : slot + 1;
+                // Group it - 2 is in its accumulator, so the promotion of group
+                // it - 4, which this slot held, is over.
+                if (it >= 2 && !mbar_wait(tfull + (it & 1), ((it - 2) >> 1) & 1, args.status, kErrTimeoutProducer, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                float* f = factors + (it % Cfg::FACTOR_SLOTS) * Cfg::FACTOR_WORDS + ft;
+                f[0] = s.x * s.z;
+                f[64] = s.y * s.z;
+                f[128] = s.x * s.w;
+                f[192] = s.y * s.w;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(tfull + (it & 1));
+            }
+        }
+        cp_async_wait<0>();
+    }
+    } else {
+        setmaxnreg_inc<Cfg::MANY_REGS>();
+        // Warps 4..11: warp w reads TMEM lane quarter w % 4 (rows 32 * (w % 4)
+        // .. + 31 of this CTA's half) and one half of the 256 columns.
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        const uint32_t lanes = uint32_t(quarter * 32) << 16;
+        uint8_t* stage = sOut + (warp - 4) * Cfg::OUT_BUFS * Cfg::OUT_BUF;
+        int it = 0, out = 0;   // groups promoted, the next stage of y
+        float* my_bias = biases + (warp - 4) * Cfg::WARP_COLS;
+        const float* my_factor = factors + half * kTileM + quarter * 32 + lane;
+        bool ok = true;
+        for (int tile = pair; ok && tile < n_tiles; tile += n_pairs) {
+            const int row0 = (tile / tiles_n) * 2 * kTileM + int(rank) * kTileM + quarter * 32;
+            const int n0 = (tile % tiles_n) * Cfg::BN + half * Cfg::WARP_COLS;
+            if (args.bias) {   // for the epilogue
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < Cfg::WARP_COLS / 32; ++i) {
+                    const int n = n0 + lane + 32 * i;
+                    cp_async4(my_bias + lane + 32 * i, args.bias + (n < args.N ? n : 0), n < args.N);
+                }
+                cp_async_commit();
+            }
+            float2 sum[Cfg::WARP_COLS / 2];
+#pragma unroll
+            for (int i = 0; i < Cfg::WARP_COLS / 2; ++i) sum[i] = make_float2(0.f, 0.f);
+#pragma unroll 1
+            for (int g = 0; g < groups; ++g, ++it) {
+                const int acc = it & 1;
+                if (!mbar_wait(tfull + acc, (it >> 1) & 1, args.status, kErrTimeoutEpilogue, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t t = tmem_base + lanes + acc * Cfg::BN + half * Cfg::WARP_COLS;
+                const float f = my_factor[(it % Cfg::FACTOR_SLOTS) * Cfg::FACTOR_WORDS];
+                // 32 columns at a time, the next 32 on their way while these are added.
+                uint32_t r[2][32];
+                tmem_ld32(t, r[0]);
+#pragma unroll
+                for (int b = 0; b < Cfg::WARP_COLS / 32; ++b) {
+                    tmem_wait_ld(r[b & 1]);
+                    if (b + 1 < Cfg::WARP_COLS / 32) {
+                        tmem_ld32(t + 32 * (b + 1), r[(b + 1) & 1]);
+                    } else {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(tempty + acc), 0));
+                    }
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        float2& a = sum[16 * b + c];
+                        a.x = fmaf(__uint_as_float(r[b & 1][2 * c]), f, a.x);
+                        a.y = fmaf(__uint_as_float(r[b & 1][2 * c + 1]), f, a.y);
+                    }
+                }
+            }
+            if (!ok) break;
+            if (n0 >= args.N || row0 >= args.M) continue;   // warp-uniform: nothing of y here
+            if (args.bias) {
+                cp_async_wait<0>();   // issued a tile ago
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < Cfg::WARP_COLS / 4; ++i) {
+                    const float4 b = *reinterpret_cast<const float4*>(my_bias + 4 * i);
+                    sum[2 * i] = __fadd2_rn(sum[2 * i], make_float2(b.x, b.y));
+                    sum[2 * i + 1] = __fadd2_rn(sum[2 * i + 1], make_float2(b.z, b.w));
+                }
+            }
+            if (args.gelu) {
+#pragma unroll
+                for (int i = 0; i < Cfg::WARP_COLS / 2; ++i) sum[i] = gelu_erf_as2(sum[i]);
+            }
+            // Each lane writes 64 bytes of its row at a time to a swizzled stage,
+            // and one TMA store per warp takes the 32 rows.  Where rows of y are not
+            // 16-byte aligned, or the last columns end inside 16 bytes (a tiled
+            // store wrote those whole: zeros behind the matrix), the warp copies
+            // the stage element by element.
+            constexpr int ELEM = OUT == kF32 ? 4 : OUT == kE4M3 ? 1 : 2;
+            constexpr int CHUNK_COLS = int(Cfg::OUT_ROW) / ELEM;
+            BlockScale bs{0.f, 0.f};
+            if constexpr (OUT == kE4M3) {
+                uint32_t a = 0;
+#pragma unroll
+                for (int i = 0; i < Cfg::WARP_COLS / 2; ++i) a = max(a, max(abs_bits(sum[i].x), abs_bits(sum[i].y)));
+                bs = block_scale(a);
+                if (row0 + lane < args.M) args.ys[int64_t(n0 / kScaleBlock) * args.ys_stride + row0 + lane] = bs.scale;
+            }
+#pragma unroll
+            for (int c = 0; c < Cfg::WARP_COLS / CHUNK_COLS; ++c) {
+                const int n = n0 + c * CHUNK_COLS;
+                if (n >= args.N) break;
+                uint8_t* buf = stage + out * Cfg::OUT_BUF;
+                out = out + 1 == Cfg::OUT_BUFS ? 0 : out + 1;
+                if (lane == 0) bulk_wait_group_read<Cfg::OUT_BUFS - 1>();   // the chunk that was in buf has left it
+                __syncwarp();
+                uint8_t* rowp = buf + lane * Cfg::OUT_ROW;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (OUT == kF32) {
+                            const float2 v = sum[c * 8 + q * 2 + i / 2];
+                            w[i] = __float_as_uint(i & 1 ? v.y : v.x);
+                        } else if constexpr (OUT == kE4M3) {
+                            const float2 v0 = sum[c * 32 + q * 8 + 2 * i], v1 = sum[c * 32 + q * 8 + 2 * i + 1];
+                            w[i] = pack_e4m3x4(v0.x * bs.inv, v0.y * bs.inv, v1.x * bs.inv, v1.y * bs.inv);
+                        } else {
+                            const float2 v = sum[c * 16 + q * 4 + i];
+                            w[i] = pack2(v.x, v.y, typename OutType<OUT>::T());
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(rowp + ((q ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                if (args.vec && (n + CHUNK_COLS <= args.N || int64_t(args.N) * ELEM % 16 == 0)) {
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) tma_store_2d(&tmY, buf, n, row0);
+                } else {
+                    __syncwarp();
+                    using T = typename OutType<OUT>::T;
+                    for (int r = 0; r < 32 && row0 + r < args.M; ++r) {
+                        T* y = static_cast<T*>(args.y) + int64_t(row0 + r) * args.y_stride;
+#pragma unroll
+                        for (int k = 0; k < (CHUNK_COLS + 31) / 32; ++k) {
+                            const int col = lane + 32 * k, byte = col * ELEM;
+                            if (col < CHUNK_COLS && n + col < args.N)
+                                y[n + col] = *reinterpret_cast<const T*>(buf + r * Cfg::OUT_ROW +
+                                                                         (((byte >> 4) ^ ((r >> 1) & 3)) << 4) + (byte & 15));
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (lane == 0) bulk_commit_group();   // one group a chunk, empty where the warp copied
+            }
+        }
+        if (lane == 0) bulk_wait_group_all();
+    }
+
+    tc_fence_before();
+    __syncwarp();
+    cluster_sync();   // no CTA leaves while its pair may still signal or read it
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, Cfg::TMEM_COLS);
+    }
+}
+
+template <int OUT>
+cudaError_t launch_pair(const GemmFp8Args& a, int num_sms, cudaStream_t stream) {
+    using Cfg = PairCfg8;
+    constexpr int ELEM = OUT == kF32 ? 4 : OUT == kE4M3 ? 1 : 2;
+    constexpr CUtensorMapDataType DT = OUT == kF32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                       : OUT == kE4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                       : OUT == kF16  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    CUtensorMap tx, tw;
+    if (!make_tmap_rows(&tx, a.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.K, a.M, a.x_stride, kStageRow, kTileM) ||
+        !make_tmap_rows(&tw, a.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.K, a.N, a.w_stride, kStageRow, kTileM))
+        return cudaErrorInvalidValue;
+    CUtensorMap ty = tx;
+    if (a.vec && !make_tmap_rows(&ty, a.y, DT, a.N, a.M, uint64_t(a.y_stride) * ELEM, Cfg::OUT_ROW / ELEM, 32,
+                                 CU_TENSOR_MAP_SWIZZLE_64B))
+        return cudaErrorInvalidValue;
+    const int64_t tiles = (int64_t(a.M) + 2 * kTileM - 1) / (2 * kTileM) * ((int64_t(a.N) + Cfg::BN - 1) / Cfg::BN);
+    if (tiles > (1 << 30)) return cudaErrorInvalidValue;
+    const int pairs = int(tiles < num_sms / 2 ? tiles : num_sms / 2);
+    gemm_fp8_pair_kernel<OUT><<<2 * pairs, Cfg::THREADS, Cfg::SMEM, stream>>>(tx, tw, ty, a);
+    return cudaGetLastError();
+}
+
 template <int OUT>
 cudaError_t launch_out(const GemmFp8Args& a, int num_sms, cudaStream_t stream) {
     if (a.M <= 16) return launch_tile<16, OUT>(a, num_sms, stream);
     if (a.M <= 32) return launch_tile<32, OUT>(a, num_sms, stream);
     if (a.M <= 64) return launch_tile<64, OUT>(a, num_sms, stream);
-    return launch_tile<128, OUT>(a, num_sms, stream);
+    if (a.M <= 2048) return launch_tile<128, OUT>(a, num_sms, stream);
+    return launch_pair<OUT>(a, num_sms, stream);
 }
 
 template <int BN, int OUT>
@@ -342,7 +746,9 @@ cudaError_t prepare_out() {
     if ((e = prepare_tile<16, OUT>()) != cudaSuccess) return e;
     if ((e = prepare_tile<32, OUT>()) != cudaSuccess) return e;
     if ((e = prepare_tile<64, OUT>()) != cudaSuccess) return e;
-    return prepare_tile<128, OUT>();
+    if ((e = prepare_tile<128, OUT>()) != cudaSuccess) return e;
+    return cudaFuncSetAttribute(gemm_fp8_pair_kernel<OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                int(PairCfg8::SMEM));
 }
 
 }  // namespace
