@@ -338,14 +338,14 @@ cudaError_t launch_tile(const GemmFp8Args& a, int num_sms, cudaStream_t stream) 
 
 struct PairCfg8 {
     static constexpr int BN = 256;
-    static constexpr int STAGES = 5;
+    static constexpr int STAGES = 4;
     static constexpr int WARPS = 8;                            // promotion and epilogue
     static constexpr int WARP_COLS = BN * 4 / WARPS;           // 128: one weight block
     static constexpr uint32_t STAGE_BYTES = 2 * kHalfBytes;    // 128 rows of x, 128 rows of w per CTA
     static constexpr uint32_t RING = STAGES * STAGE_BYTES;
-    static constexpr uint32_t OUT_ROW = 64;                    // bytes of a row of y staged at a time
+    static constexpr uint32_t OUT_ROW = 128;                   // bytes of a row of y staged at a time
     static constexpr uint32_t OUT_BUF = 32 * OUT_ROW;
-    static constexpr int OUT_BUFS = 3;                         // per warp
+    static constexpr int OUT_BUFS = 2;                         // per warp: all of a 16-bit tile
     static constexpr uint32_t OUT_BYTES = WARPS * OUT_BUFS * OUT_BUF;
     static constexpr int RAW_SLOTS = 6;                        // groups of scales on their way
     static constexpr int RAW_WORDS = 64 * 4;                   // two row and two block scales per factor thread
@@ -356,13 +356,13 @@ struct PairCfg8 {
     static constexpr size_t SMEM = RING + OUT_BYTES + SMALL_BYTES + 1024 + 256;
     // Warpgroup 0: TMA producer, UMMA issuer and two factor warps; warpgroups 1
     // and 2: promotion.  The launch gives each of the 384 threads 168 registers
-    // (64,512 in all); 128 sums and the columns in flight need more, so
-    // warpgroup 0 keeps 40 (5,120) and the others take 224 (57,344).
+    // (64,512 in all); 128 sums and 64 columns in flight need more, so
+    // warpgroup 0 keeps 72 (9,216) and the others take 216 (55,296).
     static constexpr int THREADS = 128 + 32 * WARPS;
-    static constexpr int FEW_REGS = 40, MANY_REGS = 224;
+    static constexpr int FEW_REGS = 72, MANY_REGS = 216;
     static_assert(128 * FEW_REGS + 32 * WARPS * MANY_REGS <= THREADS * 168, "the split stays within the launch");
 };
-static_assert(PairCfg8::WARP_COLS == kScaleBlock, "a warp's columns lie in one weight block");
+static_assert(PairCfg8::WARP_COLS == kScaleBlock, "a warp's columns are one weight block");
 
 template <int OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1)
@@ -378,9 +378,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
     float* factors = raw + Cfg::RAW_SLOTS * Cfg::RAW_WORDS;
     float* biases = factors + Cfg::FACTOR_SLOTS * Cfg::FACTOR_WORDS;
     uint64_t* full = reinterpret_cast<uint64_t*>(biases + Cfg::WARPS * Cfg::WARP_COLS);
-    uint64_t* empty = full + Cfg::STAGES;
-    uint64_t* tfull = empty + Cfg::STAGES;
-    uint64_t* tempty = tfull + 2;
+    uint64_t* done = full + Cfg::STAGES;
+    uint64_t* tempty = done + Cfg::STAGES;
     uint64_t* drain = tempty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -396,12 +395,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
     if (threadIdx.x == 0) {
         for (int s = 0; s < Cfg::STAGES; ++s) {
             mbar_init(full + s, 1);
-            mbar_init(empty + s, 1);
+            mbar_init(done + s, 1 + 2);              // the UMMAs and this CTA's factor warps
         }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(tfull + i, 1 + 2);             // the UMMAs and this CTA's factor warps
-            mbar_init(tempty + i, 2 * Cfg::WARPS);   // every promotion warp of the pair
-        }
+        for (int i = 0; i < 2; ++i) mbar_init(tempty + i, 2 * Cfg::WARPS);   // every promotion warp of the pair
         mbar_init(drain, 1);
         *abort_flag = 0;
         fence_barrier_init();
@@ -426,7 +422,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
                 const int m0 = (tile / tiles_n) * 2 * kTileM + int(rank) * kTileM;
                 const int n0 = (tile % tiles_n) * Cfg::BN + int(rank) * kTileM;
                 for (int g = 0; g < groups; ++g) {
-                    if (!mbar_wait(empty + s, ph ^ 1, args.status, kErrTimeoutProducer, abort_flag)) {
+                    if (!mbar_wait(done + s, ph ^ 1, args.status, kErrTimeoutProducer, abort_flag)) {
                         ok = false;
                         break;
                     }
@@ -452,7 +448,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && leader) {
+        if (leader) {
             constexpr uint32_t idesc = umma_idesc_e4m3(2 * kTileM, Cfg::BN);
             const uint64_t dX0 = umma_desc_sw128(smem_u32(sX), 16, 1024);
             const uint64_t dW0 = umma_desc_sw128(smem_u32(sW), 16, 1024);
@@ -463,19 +459,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
                 for (int g = 0; g < groups; ++g, ++it) {
                     const int acc = it & 1;
                     const uint32_t aph = (it >> 1) & 1;
-                    if (!mbar_wait(tempty + acc, aph ^ 1, args.status, kErrTimeoutMma, abort_flag) ||
-                        !mbar_wait(full + s, ph, args.status, kErrTimeoutMma, abort_flag)) {
+                    if (!mbar_wait(full + s, ph, args.status, kErrTimeoutMma, abort_flag) ||
+                        !mbar_wait(tempty + acc, aph ^ 1, args.status, kErrTimeoutMma, abort_flag)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
                     const uint64_t dx = dX0 + uint64_t(s) * (kHalfBytes >> 4), dw = dW0 + uint64_t(s) * (kHalfBytes >> 4);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        umma_f8_ss_pair(tmem_base + acc * Cfg::BN, dx + 2 * k, dw + 2 * k, idesc, k != 0);
+                        for (int k = 0; k < 4; ++k)
+                            umma_f8_ss_pair(tmem_base + acc * Cfg::BN, dx + 2 * k, dw + 2 * k, idesc, k != 0);
+                        // One commit per group (a second cost 61 clocks of the tensor
+                        // pipe): the stage is free and its sums are in the accumulator.
+                        umma_commit_pair(done + s, 0x3);
+                    }
+                    __syncwarp();
                     issued = true;
-                    umma_commit_pair(empty + s, 0x3);
-                    umma_commit_pair(tfull + acc, 0x3);
                     if (++s == Cfg::STAGES) {
                         s = 0;
                         ph ^= 1;
@@ -483,7 +483,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
                 }
             }
             if (!ok && issued) {
-                umma_commit_pair(drain, 0x1);
+                if (elect_one()) umma_commit_pair(drain, 0x1);
+                __syncwarp();
                 mbar_wait(drain, 0, args.status, kErrTimeoutDrain, nullptr);
             }
         }
@@ -491,7 +492,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
         // Factor warps: xs ws of this CTA's 128 rows and two weight blocks, for
         // each group, so that a promotion warp reads one word.  The raw scales
         // come by cp.async, RAW_SLOTS - 1 groups ahead, into words of the
-        // thread's own.  tfull of a group counts these warps too.
+        // thread's own.  A group's done barrier counts these warps too.
         const int ft = int(threadIdx.x) - 64;
         float* mine = raw + ft * 4;
         int ahead_tile = pair - n_pairs, ahead_left = 0, ahead_slot = 0;
@@ -528,41 +529,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
             }
         };
         for (int i = 0; i < Cfg::RAW_SLOTS - 1; ++i) fetch();
-        int it = 0, slot = 0;
+        int slot = 0, s = 0, lag = 0;          // lag: stage of group it - 2
+        uint32_t lag_ph = 0;
+        int it = 0;
         bool ok = true;
         for (int tile = pair; ok && tile < n_tiles; tile += n_pairs) {
             for (int g = 0; g < groups; ++g, ++it) {
                 fetch();
                 cp_async_wait<Cfg::RAW_SLOTS - 1>();
-                const float4 s = *reinterpret_cast<const float4*>(mine + slot * Cfg::RAW_WORDS);
+                const float4 v = *reinterpret_cast<const float4*>(mine + slot * Cfg::RAW_WORDS);
                 slot = slot + 1 == Cfg::RAW_SLOTS ? 0 : slot + 1;
                 // Group it - 2 is in its accumulator, so the promotion of group
                 // it - 4, which this slot held, is over.
-                if (it >= 2 && !mbar_wait(tfull + (it & 1), ((it - 2) >> 1) & 1, args.status, kErrTimeoutProducer, abort_flag)) {
-                    ok = false;
-                    break;
+                if (it >= 2) {
+                    if (!mbar_wait(done + lag, lag_ph, args.status, kErrTimeoutProducer, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    if (++lag == Cfg::STAGES) {
+                        lag = 0;
+                        lag_ph ^= 1;
+                    }
                 }
                 float* f = factors + (it % Cfg::FACTOR_SLOTS) * Cfg::FACTOR_WORDS + ft;
-                f[0] = s.x * s.z;
-                f[64] = s.y * s.z;
-                f[128] = s.x * s.w;
-                f[192] = s.y * s.w;
+                f[0] = v.x * v.z;
+                f[64] = v.y * v.z;
+                f[128] = v.x * v.w;
+                f[192] = v.y * v.w;
                 __syncwarp();
-                if (lane == 0) mbar_arrive(tfull + (it & 1));
+                if (lane == 0) mbar_arrive(done + s);
+                s = s + 1 == Cfg::STAGES ? 0 : s + 1;
             }
         }
         cp_async_wait<0>();
     }
     } else {
         setmaxnreg_inc<Cfg::MANY_REGS>();
-        // Warps 4..11: warp w reads TMEM lane quarter w % 4 (rows 32 * (w % 4)
-        // .. + 31 of this CTA's half) and one half of the 256 columns.
+        // Warp w reads TMEM lane quarter w % 4 (rows 32 * (w % 4) .. + 31 of this
+        // CTA's half) and one half of the 256 columns.
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         const uint32_t lanes = uint32_t(quarter * 32) << 16;
         uint8_t* stage = sOut + (warp - 4) * Cfg::OUT_BUFS * Cfg::OUT_BUF;
-        int it = 0, out = 0;   // groups promoted, the next stage of y
         float* my_bias = biases + (warp - 4) * Cfg::WARP_COLS;
         const float* my_factor = factors + half * kTileM + quarter * 32 + lane;
+        int it = 0, out = 0, s = 0;   // groups promoted, the next buffer of y, the group's stage
+        uint32_t ph = 0;
         bool ok = true;
         for (int tile = pair; ok && tile < n_tiles; tile += n_pairs) {
             const int row0 = (tile / tiles_n) * 2 * kTileM + int(rank) * kTileM + quarter * 32;
@@ -579,36 +590,60 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
             float2 sum[Cfg::WARP_COLS / 2];
 #pragma unroll
             for (int i = 0; i < Cfg::WARP_COLS / 2; ++i) sum[i] = make_float2(0.f, 0.f);
-#pragma unroll 1
-            for (int g = 0; g < groups; ++g, ++it) {
-                const int acc = it & 1;
-                if (!mbar_wait(tfull + acc, (it >> 1) & 1, args.status, kErrTimeoutEpilogue, abort_flag)) {
-                    ok = false;
-                    break;
+            // 64 columns on their way at a time, across groups too: the next
+            // group's first columns are asked for before the last of this one
+            // are added.  The accumulator goes back to the UMMA issuer once its
+            // last columns are in registers, before half of them are added.
+            uint32_t r[2][32];
+            float f = 0.f;
+            uint32_t t = 0;
+            auto add = [&](const uint32_t (&v)[32], int b) {
+#pragma unroll
+                for (int c = 0; c < 16; ++c)
+                    sum[16 * b + c] = packed_fma(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1]), make_float2(f, f),
+                                                 sum[16 * b + c]);
+            };
+            auto next_group = [&]() {   // waits for the next group's accumulator
+                if (!mbar_wait(done + s, ph, args.status, kErrTimeoutEpilogue, abort_flag)) return false;
+                if (++s == Cfg::STAGES) {
+                    s = 0;
+                    ph ^= 1;
                 }
                 tc_fence_after();
-                const uint32_t t = tmem_base + lanes + acc * Cfg::BN + half * Cfg::WARP_COLS;
-                const float f = my_factor[(it % Cfg::FACTOR_SLOTS) * Cfg::FACTOR_WORDS];
-                // 32 columns at a time, the next 32 on their way while these are added.
-                uint32_t r[2][32];
-                tmem_ld32(t, r[0]);
-#pragma unroll
-                for (int b = 0; b < Cfg::WARP_COLS / 32; ++b) {
-                    tmem_wait_ld(r[b & 1]);
-                    if (b + 1 < Cfg::WARP_COLS / 32) {
-                        tmem_ld32(t + 32 * (b + 1), r[(b + 1) & 1]);
-                    } else {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(tempty + acc), 0));
-                    }
-#pragma unroll
-                    for (int c = 0; c < 16; ++c) {
-                        float2& a = sum[16 * b + c];
-                        a.x = fmaf(__uint_as_float(r[b & 1][2 * c]), f, a.x);
-                        a.y = fmaf(__uint_as_float(r[b & 1][2 * c + 1]), f, a.y);
-                    }
+                t = tmem_base + lanes + (it & 1) * Cfg::BN + half * Cfg::WARP_COLS;
+                return true;
+            };
+            ok = next_group();
+            if (!ok) break;
+            tmem_ld32(t, r[0]);
+            tmem_ld32(t + 32, r[1]);
+            f = my_factor[(it % Cfg::FACTOR_SLOTS) * Cfg::FACTOR_WORDS];
+#pragma unroll 1
+            for (int g = 0; g < groups; ++g) {
+                tmem_wait_ld(r[0]);
+                tmem_wait_ld(r[1]);
+                add(r[0], 0);
+                tmem_ld32(t + 64, r[0]);
+                add(r[1], 1);
+                tmem_ld32(t + 96, r[1]);
+                tmem_wait_ld(r[0]);
+                tmem_wait_ld(r[1]);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(tempty + (it & 1)), 0));
+                ++it;
+                add(r[0], 2);
+                if (g + 1 == groups) {
+                    add(r[1], 3);
+                    break;
                 }
+                ok = next_group();
+                if (!ok) break;
+                tmem_ld32(t, r[0]);
+                const float f_next = my_factor[(it % Cfg::FACTOR_SLOTS) * Cfg::FACTOR_WORDS];
+                add(r[1], 3);
+                tmem_ld32(t + 32, r[1]);
+                f = f_next;
             }
             if (!ok) break;
             if (n0 >= args.N || row0 >= args.M) continue;   // warp-uniform: nothing of y here
@@ -626,12 +661,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
 #pragma unroll
                 for (int i = 0; i < Cfg::WARP_COLS / 2; ++i) sum[i] = gelu_erf_as2(sum[i]);
             }
-            // Each lane writes 64 bytes of its row at a time to a swizzled stage,
-            // and one TMA store per warp takes the 32 rows.  Where rows of y are not
+            // Each lane writes 128 bytes of its row at a time to a swizzled stage,
+            // and one TMA store per warp takes the 32 rows while the next tile is
+            // computed (every pair ends its tile at about the same time: stores that
+            // the warps waited for cost 2 us a tile).  Where rows of y are not
             // 16-byte aligned, or the last columns end inside 16 bytes (a tiled
             // store wrote those whole: zeros behind the matrix), the warp copies
             // the stage element by element.
-            constexpr int ELEM = OUT == kF32 ? 4 : OUT == kE4M3 ? 1 : 2;
+            using T = typename OutType<OUT>::T;
+            constexpr int ELEM = int(sizeof(T));
             constexpr int CHUNK_COLS = int(Cfg::OUT_ROW) / ELEM;
             BlockScale bs{0.f, 0.f};
             if constexpr (OUT == kE4M3) {
@@ -651,22 +689,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
                 __syncwarp();
                 uint8_t* rowp = buf + lane * Cfg::OUT_ROW;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
+                for (int q = 0; q < 8; ++q) {
                     uint32_t w[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         if constexpr (OUT == kF32) {
-                            const float2 v = sum[c * 8 + q * 2 + i / 2];
+                            const float2 v = sum[c * 16 + q * 2 + i / 2];
                             w[i] = __float_as_uint(i & 1 ? v.y : v.x);
                         } else if constexpr (OUT == kE4M3) {
-                            const float2 v0 = sum[c * 32 + q * 8 + 2 * i], v1 = sum[c * 32 + q * 8 + 2 * i + 1];
+                            const float2 v0 = sum[q * 8 + 2 * i], v1 = sum[q * 8 + 2 * i + 1];
                             w[i] = pack_e4m3x4(v0.x * bs.inv, v0.y * bs.inv, v1.x * bs.inv, v1.y * bs.inv);
                         } else {
-                            const float2 v = sum[c * 16 + q * 4 + i];
-                            w[i] = pack2(v.x, v.y, typename OutType<OUT>::T());
+                            const float2 v = sum[c * 32 + q * 4 + i];
+                            w[i] = pack2(v.x, v.y, T());
                         }
                     }
-                    *reinterpret_cast<uint4*>(rowp + ((q ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *reinterpret_cast<uint4*>(rowp + ((q ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
                 if (args.vec && (n + CHUNK_COLS <= args.N || int64_t(args.N) * ELEM % 16 == 0)) {
                     fence_proxy_async_smem();
@@ -674,15 +712,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
                     if (lane == 0) tma_store_2d(&tmY, buf, n, row0);
                 } else {
                     __syncwarp();
-                    using T = typename OutType<OUT>::T;
-                    for (int r = 0; r < 32 && row0 + r < args.M; ++r) {
-                        T* y = static_cast<T*>(args.y) + int64_t(row0 + r) * args.y_stride;
+                    for (int rr = 0; rr < 32 && row0 + rr < args.M; ++rr) {
+                        T* y = static_cast<T*>(args.y) + int64_t(row0 + rr) * args.y_stride;
 #pragma unroll
-                        for (int k = 0; k < (CHUNK_COLS + 31) / 32; ++k) {
+                        for (int k = 0; k < CHUNK_COLS / 32; ++k) {
                             const int col = lane + 32 * k, byte = col * ELEM;
-                            if (col < CHUNK_COLS && n + col < args.N)
-                                y[n + col] = *reinterpret_cast<const T*>(buf + r * Cfg::OUT_ROW +
-                                                                         (((byte >> 4) ^ ((r >> 1) & 3)) << 4) + (byte & 15));
+                            if (n + col < args.N)
+                                y[n + col] = *reinterpret_cast<const T*>(buf + rr * Cfg::OUT_ROW +
+                                                                         (((byte >> 4) ^ (rr & 7)) << 4) + (byte & 15));
                         }
                     }
                     __syncwarp();
@@ -715,8 +752,7 @@ cudaError_t launch_pair(const GemmFp8Args& a, int num_sms, cudaStream_t stream) 
         !make_tmap_rows(&tw, a.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.K, a.N, a.w_stride, kStageRow, kTileM))
         return cudaErrorInvalidValue;
     CUtensorMap ty = tx;
-    if (a.vec && !make_tmap_rows(&ty, a.y, DT, a.N, a.M, uint64_t(a.y_stride) * ELEM, Cfg::OUT_ROW / ELEM, 32,
-                                 CU_TENSOR_MAP_SWIZZLE_64B))
+    if (a.vec && !make_tmap_rows(&ty, a.y, DT, a.N, a.M, uint64_t(a.y_stride) * ELEM, Cfg::OUT_ROW / ELEM, 32))
         return cudaErrorInvalidValue;
     const int64_t tiles = (int64_t(a.M) + 2 * kTileM - 1) / (2 * kTileM) * ((int64_t(a.N) + Cfg::BN - 1) / Cfg::BN);
     if (tiles > (1 << 30)) return cudaErrorInvalidValue;

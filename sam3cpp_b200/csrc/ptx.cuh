@@ -20,6 +20,13 @@ S3T_DEV uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
+// One lane of a converged warp.
+S3T_DEV bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 S3T_DEV uint64_t globaltimer() {
     uint64_t t;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
@@ -73,16 +80,19 @@ S3T_DEV bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 
 // Bounded wait for the phase with the given parity.  Returns false (after
 // recording `code` in *status) if the phase did not complete in time, or if
-// another role of the CTA already gave up (*abort set).
+// another role of the CTA already gave up (*abort set).  The clock starts at
+// the 64th failed try: reading the global timer takes several hundred clocks,
+// which a wait of a few hundred would otherwise pay.
 S3T_DEV bool mbar_wait_limit(uint64_t* bar, uint32_t parity, int* status, int code, volatile int* abort,
                              uint64_t limit_ns) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = globaltimer();
+    uint64_t t0 = 0;
     for (uint32_t i = 1;; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 255u) == 0) {
+        if ((i & 63u) == 0) {
             if (abort && *abort) return false;
-            if (globaltimer() - t0 > limit_ns) {
+            const uint64_t now = globaltimer();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > limit_ns) {
                 report_error(status, code);
                 if (abort) *abort = 1;
                 return false;
