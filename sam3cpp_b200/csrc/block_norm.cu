@@ -8,11 +8,23 @@
 // residual stream once and the branch not at all.
 //
 // Bound by HBM: y, x and the gate are read once, x' and u written once, and a
-// row stays in registers between the two norms.  A chunk is 256 columns, eight
-// consecutive ones per lane; a row's chunks are dealt out to the warps of a
-// CTA.  A LayerNorm warp reduces its own mean and centred square sum M2 and
-// the warps' are merged by the pairwise update of Chan, Golub and LeVeque
-// (1979), so there is one exchange per norm and no cancellation.
+// row stays in registers between the two norms.  A chunk is 256 columns, two
+// groups of 128, four consecutive columns of each per lane (so that every
+// access of a warp is contiguous and a scale group's maximum is one warp
+// reduction); warp w of a row's team holds CPW consecutive chunks.
+//
+// Many rows (STREAM): persistent CTAs, four chunks a warp, so that a reduction
+// or a barrier is paid once for 32 columns a lane; the vectors wait in shared
+// memory and the rows ahead come there by bulk copies, two a warp.  82944 x
+// 1024, LayerNorm twice, gate, e4m3 out: 174 us, 5.4 TB/s; whole rows per warp
+// read straight into registers took 398 us (the loads' latency), one chunk a
+// warp with the next row in registers 269 us (four times the reductions).
+// Few rows: one chunk a warp up to 4096 columns, everything asked for at once,
+// for the latency of one row.
+//
+// A LayerNorm warp reduces its own mean and centred square sum and the warps'
+// are merged about the row's mean (Chan, Golub and LeVeque, 1979), so there is
+// one exchange per norm and no cancellation.
 #include "elements.cuh"
 #include "fp8.cuh"
 #include "kernels.h"
@@ -21,48 +33,96 @@ namespace s3t {
 
 namespace {
 
-constexpr int kChunk = 256;
-constexpr int kLaneElems = 8;
-constexpr int kMaxWarps = 16;          // of a CTA: 16 x 4 chunks hold kNormMaxDim columns
+constexpr int kChunk = 2 * kScaleBlock;
+constexpr int kMaxWarps = 16;          // of a team: 16 x 4 chunks hold kNormMaxDim columns
+constexpr int kSlots = 2;              // rows ahead (STREAM)
+constexpr int kStreamCpw = 4;
+constexpr int kStreamWarps = 12;
+constexpr int kStreamBytes = 220 * 1024;
+constexpr int kVectors = 5;            // post weight and bias, branch factor, pre weight and bias
 
-// Columns of a lane's eight elements of a chunk: consecutive (VEC), or 16
-// apart within the lane's half-warp group of 128, so that scalar accesses of
-// a half warp still cover consecutive addresses.
+// A lane's eight elements of a chunk are two quads: quad h is columns
+// h * 128 + 4 lane .. + 3 (VEC: whole or not there at all), or h * 128 + lane +
+// 32 i where rows are not aligned.
 template <bool VEC>
-S3T_DEV int chunk_col(int lane, int i) {
-    return VEC ? lane * kLaneElems + i : (lane >> 4) * kScaleBlock + (lane & 15) + 16 * i;
+S3T_DEV int quad_col(int lane, int h, int i) {
+    return h * kScaleBlock + (VEC ? lane * 4 + i : lane + 32 * i);
 }
 
+template <typename T>
+S3T_DEV void widen4(const T* p, float2& a, float2& b) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        a = make_float2(v.x, v.y);
+        b = make_float2(v.z, v.w);
+    } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        a = unpack2(v.x, T());
+        b = unpack2(v.y, T());
+    }
+}
+
+// A lane's elements of the chunk at p (columns c0 ..), zeros past dim.
 template <bool VEC, typename T>
-S3T_DEV void load_chunk(const T* p, int c0, int dim, int lane, float (&v)[kLaneElems]) {
-    if (VEC) {
-        if (c0 + lane * kLaneElems < dim) {
-            load8(p + c0 + lane * kLaneElems, v);
-            return;
+S3T_DEV void load_chunk(const T* p, int c0, int dim, int lane, float2 (&v)[4]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if constexpr (VEC) {
+            const int c = c0 + quad_col<true>(lane, h, 0);
+            if (c < dim) widen4(p + c, v[2 * h], v[2 * h + 1]);
+            else v[2 * h] = v[2 * h + 1] = make_float2(0.f, 0.f);
+        } else {
+            float f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = c0 + quad_col<false>(lane, h, i);
+                f[i] = c < dim ? to_float(p[c]) : 0.f;
+            }
+            v[2 * h] = make_float2(f[0], f[1]);
+            v[2 * h + 1] = make_float2(f[2], f[3]);
         }
-#pragma unroll
-        for (int i = 0; i < kLaneElems; ++i) v[i] = 0.f;
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < kLaneElems; ++i) {
-        const int c = c0 + chunk_col<VEC>(lane, i);
-        v[i] = c < dim ? to_float(p[c]) : 0.f;
     }
 }
 
 template <bool VEC, typename T>
-S3T_DEV void store_chunk(T* p, int c0, int dim, int lane, const float (&v)[kLaneElems]) {
-    if (VEC) {
-        if (c0 + lane * kLaneElems < dim) store8(p + c0 + lane * kLaneElems, v);
-        return;
-    }
+S3T_DEV void store_chunk(T* p, int c0, int dim, int lane, const float2 (&v)[4]) {
 #pragma unroll
-    for (int i = 0; i < kLaneElems; ++i) {
-        const int c = c0 + chunk_col<VEC>(lane, i);
-        if (c < dim) p[c] = from_float<T>(v[i]);
+    for (int h = 0; h < 2; ++h) {
+        const float2 a = v[2 * h], b = v[2 * h + 1];
+        if constexpr (VEC) {
+            const int c = c0 + quad_col<true>(lane, h, 0);
+            if (c >= dim) continue;
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p + c) = make_float4(a.x, a.y, b.x, b.y);
+            else *reinterpret_cast<uint2*>(p + c) = make_uint2(pack2(a.x, a.y, T()), pack2(b.x, b.y, T()));
+        } else {
+            const float f[4] = {a.x, a.y, b.x, b.y};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = c0 + quad_col<false>(lane, h, i);
+                if (c < dim) p[c] = from_float<T>(f[i]);
+            }
+        }
     }
 }
+
+// Element k of vector p: `otherwise` where there is none, 0 past the last
+// column (so that columns past dim add nothing to x' and u).
+template <bool VEC>
+S3T_DEV void load_vector(const float* p, float otherwise, int c0, int dim, int lane, float2 (&v)[4]) {
+    if (p) {
+        load_chunk<VEC>(p, c0, dim, lane, v);
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                v[2 * h + i].x = c0 + quad_col<VEC>(lane, h, 2 * i) < dim ? otherwise : 0.f;
+                v[2 * h + i].y = c0 + quad_col<VEC>(lane, h, 2 * i + 1) < dim ? otherwise : 0.f;
+            }
+    }
+}
+
+S3T_DEV float2 both(float v) { return make_float2(v, v); }
 
 S3T_DEV float warp_sum(float v) {
 #pragma unroll
@@ -70,211 +130,409 @@ S3T_DEV float warp_sum(float v) {
     return v;
 }
 
-// Mean (0 for RMSNorm) and 1 / sqrt(mean square or variance + eps) of a row
-// whose chunks c = warp, warp + WARPS, ... this warp holds; columns past dim
-// hold 0.
 struct RowStats {
     float mean, rstd;
 };
 
+// How a row lies on the warps of its team: warp w holds the columns from
+// w * CPW * kChunk on, all of them full but the last warp's.
+struct Split {
+    int lane, warp, warps, team;
+    int last;                         // columns of the last warp
+    float inv_dim, inv_last;
+};
+
+// Barrier of one team's warps (named barrier 1 + team).
+S3T_DEV void team_sync(const Split& sp) {
+    asm volatile("bar.sync %0, %1;" ::"r"(sp.team + 1), "r"(sp.warps * 32) : "memory");
+}
+
+// Mean (0 for RMSNorm) and 1 / sqrt(mean square or variance + eps) of a row of
+// which this warp holds v, zeros past dim.
 template <int CPW, bool VEC>
-S3T_DEV RowStats row_stats(const float (&v)[CPW][kLaneElems], int layer, int dim, float eps, int warp, int warps, int lane,
-                           float2* exchange) {
-    float n = 0.f, mean = 0.f, m2 = 0.f;
+S3T_DEV RowStats row_stats(const float2 (&v)[CPW][4], int layer, int dim, float eps, const Split& sp, float2* exchange) {
+    constexpr float kFull = float(CPW * kChunk);
+    float sum = 0.f, mean = 0.f;
     if (layer) {
-        float s = 0.f;
-        int held = 0;
+        float2 t = v[0][0];
 #pragma unroll
-        for (int j = 0; j < CPW; ++j) {
-            const int c0 = (warp + j * warps) * kChunk;
-            held += max(0, min(kChunk, dim - c0));
+        for (int j = 0; j < CPW; ++j)
 #pragma unroll
-            for (int i = 0; i < kLaneElems; ++i) s += v[j][i];
-        }
-        n = float(held);
-        mean = held ? warp_sum(s) / n : 0.f;
+            for (int i = j == 0 ? 1 : 0; i < 4; ++i) t = __fadd2_rn(t, v[j][i]);
+        sum = warp_sum(t.x + t.y);
+        mean = sum * (sp.warp + 1 == sp.warps ? sp.inv_last : 1.f / kFull);
     }
+    float2 q = both(0.f);
+    const float2 minus = both(-mean);
 #pragma unroll
     for (int j = 0; j < CPW; ++j) {
-        const int c0 = (warp + j * warps) * kChunk;
+        const int c0 = (sp.warp * CPW + j) * kChunk;
+        if (!layer || c0 + kChunk <= dim) {
 #pragma unroll
-        for (int i = 0; i < kLaneElems; ++i) {
-            const float d = v[j][i] - mean;
-            if (!layer || c0 + chunk_col<VEC>(lane, i) < dim) m2 = fmaf(d, d, m2);
+            for (int i = 0; i < 4; ++i) {
+                const float2 d = __fadd2_rn(v[j][i], minus);
+                q = __ffma2_rn(d, d, q);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float2 d = __fadd2_rn(v[j][i], minus);
+                if (c0 + quad_col<VEC>(sp.lane, i / 2, 2 * (i & 1)) >= dim) d.x = 0.f;
+                if (c0 + quad_col<VEC>(sp.lane, i / 2, 2 * (i & 1) + 1) >= dim) d.y = 0.f;
+                q = __ffma2_rn(d, d, q);
+            }
         }
     }
-    m2 = warp_sum(m2);
-    if (warps > 1) {
-        __syncthreads();   // the exchange of the norm before has been read
-        if (lane == 0) exchange[warp] = make_float2(mean, m2);
-        __syncthreads();
-        // Every warp merges all partials in the same order.
-        n = mean = m2 = 0.f;
-        for (int w = 0; w < warps; ++w) {
+    float m2 = warp_sum(q.x + q.y);
+    if (sp.warps > 1) {
+        if (sp.lane == 0) exchange[sp.warp] = make_float2(sum, m2);
+        team_sync(sp);
+        // Every warp merges all partials in the same order: the squares about
+        // the row's mean are those about each warp's plus the means' spread.
+        float total = 0.f;
+        m2 = 0.f;
+#pragma unroll 4
+        for (int w = 0; w < sp.warps; ++w) {
             const float2 e = exchange[w];
-            if (!layer) {
-                m2 += e.y;
-                continue;
+            total += e.x;
+            m2 += e.y;
+        }
+        if (layer) {
+            mean = total * sp.inv_dim;
+#pragma unroll 4
+            for (int w = 0; w + 1 < sp.warps; ++w) {
+                const float d = fmaf(exchange[w].x, 1.f / kFull, -mean);
+                m2 = fmaf(d * kFull, d, m2);
             }
-            int held = 0;
-#pragma unroll
-            for (int j = 0; j < CPW; ++j) held += max(0, min(kChunk, dim - (w + j * warps) * kChunk));
-            const float nb = float(held);
-            if (nb == 0.f) continue;
-            const float d = e.x - mean, nn = n + nb;
-            m2 += e.y + d * d * (n * nb / nn);
-            mean += d * (nb / nn);
-            n = nn;
+            const float d = fmaf(exchange[sp.warps - 1].x, sp.inv_last, -mean);
+            m2 = fmaf(d * float(sp.last), d, m2);
         }
     }
-    return {mean, rsqrtf(m2 / float(dim) + eps)};
+    return {mean, rsqrtf(fmaf(m2, sp.inv_dim, eps))};
 }
 
-template <bool VEC>
-S3T_DEV void load_weight(const float* w, float otherwise, int c0, int dim, int lane, float (&v)[kLaneElems]) {
-    if (w) {
-        load_chunk<VEC>(w, c0, dim, lane, v);
-    } else {
+// v = (v - mean) rstd w + b
+S3T_DEV void normalize(float2 (&v)[4], RowStats st, const float2 (&w)[4], const float2 (&b)[4]) {
 #pragma unroll
-        for (int i = 0; i < kLaneElems; ++i) v[i] = otherwise;
+    for (int i = 0; i < 4; ++i)
+        v[i] = __ffma2_rn(__fmul2_rn(__fadd2_rn(v[i], both(-st.mean)), both(st.rstd)), w[i], b[i]);
+}
+
+S3T_DEV void apply_gate(float2 (&h)[4], float2 (&g)[4], int act) {
+    if (act == kGateSigmoid) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g[i] = make_float2(1.f / (1.f + expf(-g[i].x)), 1.f / (1.f + expf(-g[i].y)));
+    } else if (act == kGateTanh) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g[i] = make_float2(tanhf(g[i].x), tanhf(g[i].y));
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __fmul2_rn(h[i], g[i]);
 }
 
-// A CTA takes blockDim.y rows, each by blockDim.x / 32 warps (blockDim.y = 1
-// where a row has more than one warp).
-template <typename T, typename R, int CPW, bool VEC>
-__global__ void __launch_bounds__(32 * kMaxWarps) norm_residual_kernel(const NormResidualArgs a) {
-    __shared__ float2 exchange[kMaxWarps];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int64_t row = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
-    if (row >= a.rows) return;   // whole rows: no barrier is shared between rows
-    const int dim = a.dim;
-    const R* xr = static_cast<const R*>(a.x) + row * a.x_stride;
-    float x[CPW][kLaneElems], h[CPW][kLaneElems];
+// u of this warp's chunks in 8 bits, with the scales of their groups.
+template <int CPW, bool VEC>
+S3T_DEV void store_eight(const NormResidualArgs& a, uint32_t row, int c0, int lane, float2 (&v)[CPW][4]) {
+    // Columns past dim are zeros: their weights are.
+    uint32_t peak[2 * CPW];
 #pragma unroll
-    for (int j = 0; j < CPW; ++j) load_chunk<VEC>(xr, (warp + j * warps) * kChunk, dim, lane, x[j]);
-    if (a.y) {
-        const T* yr = static_cast<const T*>(a.y) + row * a.y_stride;
+    for (int k = 0; k < 2 * CPW; ++k) {
+        const float2 p = v[k / 2][2 * (k & 1)], q = v[k / 2][2 * (k & 1) + 1];
+        peak[k] = __reduce_max_sync(0xffffffffu, max(max(abs_bits(p.x), abs_bits(p.y)), max(abs_bits(q.x), abs_bits(q.y))));
+    }
+    // Lane 2 k divides for group k's scale, lane 2 k + 1 for its inverse.
+    uint32_t pick = peak[0];
 #pragma unroll
-        for (int j = 0; j < CPW; ++j) load_chunk<VEC>(yr, (warp + j * warps) * kChunk, dim, lane, h[j]);
-        if (a.post) {
-            const RowStats st = row_stats<CPW, VEC>(h, a.layer, dim, a.eps, warp, warps, lane, exchange);
+    for (int k = 1; k < 2 * CPW; ++k)
+        if ((lane >> 1) == k) pick = peak[k];
+    const float top = __uint_as_float(max(pick, kAmaxFloorBits));
+    const bool odd = lane & 1;
+    const float quotient = __fdiv_rn(odd ? kE4M3Max : top, odd ? top : kE4M3Max);
+    uint8_t* q = static_cast<uint8_t*>(a.u) + int64_t(row) * a.u_stride;
 #pragma unroll
-            for (int j = 0; j < CPW; ++j) {
-                const int c0 = (warp + j * warps) * kChunk;
-                float w[kLaneElems], b[kLaneElems];
-                load_weight<VEC>(a.post_weight, 1.f, c0, dim, lane, w);
-                load_weight<VEC>(a.post_bias, 0.f, c0, dim, lane, b);
+    for (int k = 0; k < 2 * CPW; ++k) {
+        const float2 inv = both(__shfl_sync(0xffffffffu, quotient, 2 * k + 1));
+        const float2 s = __fmul2_rn(v[k / 2][2 * (k & 1)], inv), t = __fmul2_rn(v[k / 2][2 * (k & 1) + 1], inv);
+        const uint32_t codes = pack_e4m3x4(s.x, s.y, t.x, t.y);
+        const int base = c0 + (k / 2) * kChunk;
+        if constexpr (VEC) {
+            const int c = base + quad_col<true>(lane, k & 1, 0);
+            if (c < a.dim) *reinterpret_cast<uint32_t*>(q + c) = codes;
+        } else {
 #pragma unroll
-                for (int i = 0; i < kLaneElems; ++i) h[j][i] = fmaf((h[j][i] - st.mean) * st.rstd, w[i], b[i]);
+            for (int i = 0; i < 4; ++i) {
+                const int c = base + quad_col<false>(lane, k & 1, i);
+                if (c < a.dim) q[c] = uint8_t(codes >> (8 * i));
             }
+        }
+    }
+    const int g = c0 + (lane >> 1) * kScaleBlock;
+    if (!odd && lane < 4 * CPW && g < a.dim) a.u_scale[int64_t(g / kScaleBlock) * a.u_scale_stride + row] = quotient;
+}
+
+// Few rows: a team of blockDim.x / 32 warps takes one row, blockDim.y teams a CTA.
+template <typename T, typename R, int CPW, bool VEC>
+__global__ void __launch_bounds__(32 * kMaxWarps) norm_rows_kernel(const NormResidualArgs a) {
+    __shared__ float2 exchange[4][2][kMaxWarps];
+    constexpr bool KEEP = CPW == 1;      // the vectors fit registers: asked for with the row
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, team = threadIdx.y;
+    const int dim = a.dim, last = dim - (warps - 1) * CPW * kChunk;
+    const Split sp{lane, warp, warps, team, last, 1.f / float(dim), 1.f / float(last)};
+    const uint32_t row = blockIdx.x * blockDim.y + team;
+    if (row >= uint32_t(a.rows)) return;   // a whole team: no barrier is shared between teams
+    const int c0 = warp * CPW * kChunk;
+    float2 x[CPW][4], h[CPW][4], g[CPW][4], vec[kVectors][4];
+    auto vectors = [&](int k, const float* p, float otherwise, int j) {
+        load_vector<VEC>(p, otherwise, c0 + j * kChunk, dim, lane, vec[k]);
+    };
+#pragma unroll
+    for (int j = 0; j < CPW; ++j) {
+        load_chunk<VEC>(static_cast<const R*>(a.x) + int64_t(row) * a.x_stride, c0 + j * kChunk, dim, lane, x[j]);
+        if (a.y) load_chunk<VEC>(static_cast<const T*>(a.y) + int64_t(row) * a.y_stride, c0 + j * kChunk, dim, lane, h[j]);
+        if (KEEP && a.gate)
+            load_chunk<VEC>(static_cast<const T*>(a.gate) + int64_t(row / uint32_t(a.gate_rows)) * a.gate_stride,
+                            c0 + j * kChunk, dim, lane, g[j]);
+    }
+    if (KEEP) {
+        vectors(0, a.post_weight, 1.f, 0);
+        vectors(1, a.post_bias, 0.f, 0);
+        vectors(2, a.channel, 1.f, 0);
+        vectors(3, a.pre_weight, 1.f, 0);
+        vectors(4, a.pre_bias, 0.f, 0);
+    }
+    RowStats st{0.f, 1.f};
+    if (a.post) st = row_stats<CPW, VEC>(h, a.layer, dim, a.eps, sp, exchange[team][0]);
+#pragma unroll
+    for (int j = 0; j < CPW; ++j) {
+        if (a.post) {
+            if (!KEEP) {
+                vectors(0, a.post_weight, 1.f, j);
+                vectors(1, a.post_bias, 0.f, j);
+            }
+            normalize(h[j], st, vec[0], vec[1]);
         }
         if (a.gate) {
-            const T* gr = static_cast<const T*>(a.gate) + (uint32_t(row) / uint32_t(a.gate_rows)) * a.gate_stride;
+            if (!KEEP)
+                load_chunk<VEC>(static_cast<const T*>(a.gate) + int64_t(row / uint32_t(a.gate_rows)) * a.gate_stride,
+                                c0 + j * kChunk, dim, lane, g[j]);
+            apply_gate(h[j], g[j], a.gate_act);
+        }
+        if (!KEEP) vectors(2, a.channel, 1.f, j);
 #pragma unroll
-            for (int j = 0; j < CPW; ++j) {
-                float g[kLaneElems];
-                load_chunk<VEC>(gr, (warp + j * warps) * kChunk, dim, lane, g);
+        for (int i = 0; i < 4; ++i) {
+            x[j][i] = __fmul2_rn(x[j][i], both(a.resid_scale));
+            if (a.y) x[j][i] = __ffma2_rn(__fmul2_rn(vec[2][i], both(a.branch_scale)), h[j][i], x[j][i]);
+        }
+        if (a.x_out)
+            store_chunk<VEC>(static_cast<R*>(a.x_out) + int64_t(row) * a.x_out_stride, c0 + j * kChunk, dim, lane, x[j]);
+    }
+    if (!a.u) return;
+    st = row_stats<CPW, VEC>(x, a.layer, dim, a.eps, sp, exchange[team][1]);
 #pragma unroll
-                for (int i = 0; i < kLaneElems; ++i) {
-                    if (a.gate_act == kGateSigmoid) g[i] = 1.f / (1.f + expf(-g[i]));
-                    if (a.gate_act == kGateTanh) g[i] = tanhf(g[i]);
-                    h[j][i] *= g[i];
+    for (int j = 0; j < CPW; ++j) {
+        if (!KEEP) {
+            vectors(3, a.pre_weight, 1.f, j);
+            vectors(4, a.pre_bias, 0.f, j);
+        }
+        normalize(x[j], st, vec[3], vec[4]);
+        if (!a.u_eight)
+            store_chunk<VEC>(static_cast<T*>(a.u) + int64_t(row) * a.u_stride, c0 + j * kChunk, dim, lane, x[j]);
+    }
+    if (a.u_eight) store_eight<CPW, VEC>(a, row, c0, lane, x);
+}
+
+// Shared memory of a streaming CTA: the vectors, each a row of floats padded
+// to its team's columns; then per warp kSlots rows of its columns of x, y and
+// gate; then the barriers.
+template <typename T, typename R>
+struct StreamRow {
+    static constexpr uint32_t COLS = kStreamCpw * kChunk;
+    static constexpr uint32_t X = COLS * sizeof(R), Y = COLS * sizeof(T);
+    static constexpr uint32_t BYTES = X + 2 * Y;
+};
+
+template <typename T, typename R>
+__global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const NormResidualArgs a) {
+    constexpr int CPW = kStreamCpw;
+    using Row = StreamRow<T, R>;
+    // Two parities: a slot is written again two barriers after its last read.
+    __shared__ float2 exchange[kStreamWarps][2][2][kStreamWarps];
+    __shared__ uint64_t arrived[kStreamWarps][kSlots];
+    extern __shared__ uint4 words[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, team = threadIdx.y;
+    const int thread = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
+    const int dim = a.dim, last = dim - (warps - 1) * int(Row::COLS), padded = warps * int(Row::COLS);
+    const Split sp{lane, warp, warps, team, last, 1.f / float(dim), 1.f / float(last)};
+    const int c0 = warp * int(Row::COLS), cols = warp + 1 == warps ? last : int(Row::COLS);
+    float* vec = reinterpret_cast<float*>(words);
+    {
+        const float* const from[kVectors] = {a.post_weight, a.post_bias, a.channel, a.pre_weight, a.pre_bias};
+#pragma unroll
+        for (int k = 0; k < kVectors; ++k) {
+            const float otherwise = k == 1 || k == 4 ? 0.f : 1.f, times = k == 2 ? a.branch_scale : 1.f;
+            for (int c = thread; c < padded; c += threads)
+                vec[k * padded + c] = c < dim ? (from[k] ? from[k][c] : otherwise) * times : 0.f;
+        }
+    }
+    // Columns past dim are never copied: they stay zeros.
+    uint8_t* mine = reinterpret_cast<uint8_t*>(vec + kVectors * padded) + (team * warps + warp) * kSlots * Row::BYTES;
+    for (uint32_t i = lane; i < kSlots * Row::BYTES / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
+    uint64_t* bar = arrived[team * warps + warp];
+    if (lane == 0) {
+        for (int i = 0; i < kSlots; ++i) mbar_init(bar + i, 1);
+        fence_barrier_init();
+    }
+    fence_proxy_async_smem();
+    __syncthreads();
+
+    const uint32_t rows = uint32_t(a.rows), stride = gridDim.x * blockDim.y;
+    uint32_t row = blockIdx.x * blockDim.y + team;
+    const R* xp = static_cast<const R*>(a.x) + int64_t(row) * a.x_stride + c0;
+    const T* yp = static_cast<const T*>(a.y) + int64_t(row) * a.y_stride + c0;
+    R* xo = static_cast<R*>(a.x_out) + int64_t(row) * a.x_out_stride + c0;
+    const int64_t x_step = int64_t(stride) * a.x_stride, y_step = int64_t(stride) * a.y_stride,
+                  xo_step = int64_t(stride) * a.x_out_stride;
+    uint32_t ahead = row;
+    auto fetch = [&](int slot) {       // one lane
+        if (ahead >= rows) return;
+        uint8_t* to = mine + slot * Row::BYTES;
+        mbar_arrive_expect_tx(bar + slot, uint32_t(cols) * (sizeof(R) + (a.y ? sizeof(T) : 0) + (a.gate ? sizeof(T) : 0)));
+        if (a.y) bulk_load(to + Row::X, yp, cols * sizeof(T), bar + slot);
+        bulk_load(to, xp, cols * sizeof(R), bar + slot);
+        if (a.gate)
+            bulk_load(to + Row::X + Row::Y,
+                      static_cast<const T*>(a.gate) + int64_t(ahead / uint32_t(a.gate_rows)) * a.gate_stride + c0,
+                      cols * sizeof(T), bar + slot);
+        xp += x_step;
+        yp += y_step;
+        ahead = rows - ahead > stride ? ahead + stride : rows;
+    };
+    if (lane == 0)
+        for (int i = 0; i < kSlots; ++i) fetch(i);
+    const bool whole = c0 + int(Row::COLS) <= dim;      // no column of this warp lies past dim
+    bool lost = false;
+    for (uint32_t it = 0; row < rows; ++it) {
+        const int slot = it & 1;
+        // A row that never came is reported; the loop goes on without waiting, so
+        // that no warp of the team is left alone at a barrier.
+        lost = lost || !mbar_wait(bar + slot, (it >> 1) & 1, a.status, kErrTimeoutProducer, nullptr);
+        const uint8_t* from = mine + slot * Row::BYTES;
+        float2 x[CPW][4], h[CPW][4];
+        auto vector = [&](int k, int j, float2(&v)[4]) { load_chunk<true>(vec + k * padded + c0 + j * kChunk, 0, kChunk, lane, v); };
+        if (a.y) {
+#pragma unroll
+            for (int j = 0; j < CPW; ++j)
+                load_chunk<true>(reinterpret_cast<const T*>(from + Row::X) + j * kChunk, 0, kChunk, lane, h[j]);
+            if (a.post) {
+                const RowStats st = row_stats<CPW, true>(h, a.layer, dim, a.eps, sp, exchange[team][it & 1][0]);
+#pragma unroll
+                for (int j = 0; j < CPW; ++j) {
+                    float2 w[4], b[4];
+                    vector(0, j, w);
+                    vector(1, j, b);
+                    normalize(h[j], st, w, b);
+                }
+            }
+            if (a.gate) {
+#pragma unroll
+                for (int j = 0; j < CPW; ++j) {
+                    float2 g[4];
+                    load_chunk<true>(reinterpret_cast<const T*>(from + Row::X + Row::Y) + j * kChunk, 0, kChunk, lane, g);
+                    apply_gate(h[j], g, a.gate_act);
                 }
             }
         }
 #pragma unroll
         for (int j = 0; j < CPW; ++j) {
-            const int c0 = (warp + j * warps) * kChunk;
-            float ch[kLaneElems];
-            load_weight<VEC>(a.channel, 1.f, c0, dim, lane, ch);
+            load_chunk<true>(reinterpret_cast<const R*>(from) + j * kChunk, 0, kChunk, lane, x[j]);
+            if (a.y) {
+                float2 s[4];
+                vector(2, j, s);
 #pragma unroll
-            for (int i = 0; i < kLaneElems; ++i) {
-                // Columns past dim stay out of the row's sums.
-                const bool in = c0 + chunk_col<VEC>(lane, i) < dim;
-                x[j][i] = in ? fmaf(a.branch_scale * ch[i], h[j][i], a.resid_scale * x[j][i]) : 0.f;
+                for (int i = 0; i < 4; ++i) x[j][i] = __ffma2_rn(both(a.resid_scale), x[j][i], __fmul2_rn(s[i], h[j][i]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[j][i] = __fmul2_rn(both(a.resid_scale), x[j][i]);
             }
         }
-    } else {
+        __syncwarp();
+        if (lane == 0) fetch(slot);   // every lane has read the slot
+        if (a.x_out) {
 #pragma unroll
-        for (int j = 0; j < CPW; ++j)
-#pragma unroll
-            for (int i = 0; i < kLaneElems; ++i) x[j][i] *= a.resid_scale;
-    }
-    if (a.x_out) {
-        R* xo = static_cast<R*>(a.x_out) + row * a.x_out_stride;
-#pragma unroll
-        for (int j = 0; j < CPW; ++j) store_chunk<VEC>(xo, (warp + j * warps) * kChunk, dim, lane, x[j]);
-    }
-    if (!a.u) return;
-    const RowStats st = row_stats<CPW, VEC>(x, a.layer, dim, a.eps, warp, warps, lane, exchange);
-#pragma unroll
-    for (int j = 0; j < CPW; ++j) {
-        const int c0 = (warp + j * warps) * kChunk;
-        float w[kLaneElems], b[kLaneElems];
-        load_weight<VEC>(a.pre_weight, 1.f, c0, dim, lane, w);
-        load_weight<VEC>(a.pre_bias, 0.f, c0, dim, lane, b);
-#pragma unroll
-        for (int i = 0; i < kLaneElems; ++i) w[i] = fmaf((x[j][i] - st.mean) * st.rstd, w[i], b[i]);
-        if (!a.u_eight) {
-            store_chunk<VEC>(static_cast<T*>(a.u) + row * a.u_stride, c0, dim, lane, w);
-            continue;
-        }
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < kLaneElems; ++i)
-            if (c0 + chunk_col<VEC>(lane, i) < dim) m = max(m, abs_bits(w[i]));
-#pragma unroll
-        for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const BlockScale s = block_scale(m);
-        uint8_t* q = static_cast<uint8_t*>(a.u) + row * a.u_stride;
-        const uint32_t lo = pack_e4m3x4(w[0] * s.inv, w[1] * s.inv, w[2] * s.inv, w[3] * s.inv);
-        const uint32_t hi = pack_e4m3x4(w[4] * s.inv, w[5] * s.inv, w[6] * s.inv, w[7] * s.inv);
-        if (VEC) {
-            if (c0 + lane * kLaneElems < dim) *reinterpret_cast<uint2*>(q + c0 + lane * kLaneElems) = make_uint2(lo, hi);
-        } else {
-#pragma unroll
-            for (int i = 0; i < kLaneElems; ++i) {
-                const int c = c0 + chunk_col<VEC>(lane, i);
-                if (c < dim) q[c] = uint8_t((i < 4 ? lo : hi) >> (8 * (i & 3)));
+            for (int j = 0; j < CPW; ++j) {
+                if (whole) store_chunk<true>(xo + j * kChunk, 0, kChunk, lane, x[j]);
+                else store_chunk<true>(xo, j * kChunk, cols, lane, x[j]);
             }
         }
-        const int g0 = c0 + (lane >> 4) * kScaleBlock;
-        if ((lane & 15) == 0 && g0 < dim) a.u_scale[int64_t(g0 / kScaleBlock) * a.u_scale_stride + row] = s.scale;
+        if (a.u) {
+            const RowStats st = row_stats<CPW, true>(x, a.layer, dim, a.eps, sp, exchange[team][it & 1][1]);
+#pragma unroll
+            for (int j = 0; j < CPW; ++j) {
+                float2 w[4], b[4];
+                vector(3, j, w);
+                vector(4, j, b);
+                normalize(x[j], st, w, b);
+                if (!a.u_eight)
+                    store_chunk<true>(static_cast<T*>(a.u) + int64_t(row) * a.u_stride, c0 + j * kChunk, dim, lane, x[j]);
+            }
+            if (a.u_eight) store_eight<CPW, true>(a, row, c0, lane, x);
+        }
+        xo += xo_step;
+        row = rows - row > stride ? row + stride : rows;
     }
 }
 
-template <typename T, typename R, int CPW>
-cudaError_t launch_cpw(const NormResidualArgs& a, dim3 grid, dim3 block, cudaStream_t stream) {
-    if (a.vec) norm_residual_kernel<T, R, CPW, true><<<grid, block, 0, stream>>>(a);
-    else norm_residual_kernel<T, R, CPW, false><<<grid, block, 0, stream>>>(a);
+template <typename T, typename R, int CPW, bool VEC>
+cudaError_t launch_few(const NormResidualArgs& a, cudaStream_t stream) {
+    const int warps = (a.dim + CPW * kChunk - 1) / (CPW * kChunk);
+    const int teams = warps == 1 ? 4 : 1;
+    const int64_t ctas = (a.rows + teams - 1) / teams;
+    norm_rows_kernel<T, R, CPW, VEC><<<uint32_t(ctas), dim3(32 * warps, teams), 0, stream>>>(a);
     return cudaGetLastError();
 }
 
 template <typename T, typename R>
-cudaError_t launch_types(const NormResidualArgs& a, cudaStream_t stream) {
-    const int chunks = (a.dim + kChunk - 1) / kChunk;
-    // Many rows: as few warps a row as hold it, for whole rows in flight
-    // without barriers.  Few rows: one chunk a warp, for latency.
-    const int cpw = a.rows >= 2048 || chunks > 16 ? 4 : 1;
-    const int warps = (chunks + cpw - 1) / cpw;
-    const int rows_per_cta = warps == 1 ? 4 : 1;
-    const int64_t ctas = (a.rows + rows_per_cta - 1) / rows_per_cta;
-    if (ctas > 0x7fffffff || warps > kMaxWarps) return cudaErrorInvalidValue;
-    const dim3 grid{uint32_t(ctas)}, block(32 * warps, rows_per_cta);
-    return cpw == 4 ? launch_cpw<T, R, 4>(a, grid, block, stream) : launch_cpw<T, R, 1>(a, grid, block, stream);
+cudaError_t launch_types(const NormResidualArgs& a, int num_sms, cudaStream_t stream) {
+    using Row = StreamRow<T, R>;
+    const int warps = (a.dim + int(Row::COLS) - 1) / int(Row::COLS);
+    const int vector_bytes = kVectors * warps * int(Row::COLS) * 4;
+    int teams = vector_bytes < kStreamBytes ? (kStreamBytes - vector_bytes) / (warps * kSlots * int(Row::BYTES)) : 0;
+    if (teams > kStreamWarps / warps) teams = kStreamWarps / warps;
+    // Two rows a team and more: the rows ahead pay for the set-up.
+    if (a.vec && teams > 0 && a.rows >= int64_t(2) * num_sms * teams) {
+        norm_stream_kernel<T, R><<<num_sms, dim3(32 * warps, teams),
+                                   uint32_t(vector_bytes) + uint32_t(teams * warps) * kSlots * Row::BYTES, stream>>>(a);
+        return cudaGetLastError();
+    }
+    if (a.dim <= kMaxWarps * kChunk) return a.vec ? launch_few<T, R, 1, true>(a, stream) : launch_few<T, R, 1, false>(a, stream);
+    return a.vec ? launch_few<T, R, 4, true>(a, stream) : launch_few<T, R, 4, false>(a, stream);
+}
+
+template <typename T, typename R>
+cudaError_t prepare_types() {
+    return cudaFuncSetAttribute(norm_stream_kernel<T, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamBytes);
 }
 
 }  // namespace
 
-cudaError_t launch_norm_residual(const NormResidualArgs& a, cudaStream_t stream) {
+cudaError_t norm_prepare() {
+    cudaError_t e;
+    if ((e = prepare_types<float, float>()) != cudaSuccess) return e;
+    if ((e = prepare_types<__half, float>()) != cudaSuccess) return e;
+    if ((e = prepare_types<__half, __half>()) != cudaSuccess) return e;
+    if ((e = prepare_types<__nv_bfloat16, float>()) != cudaSuccess) return e;
+    return prepare_types<__nv_bfloat16, __nv_bfloat16>();
+}
+
+cudaError_t launch_norm_residual(const NormResidualArgs& a, int num_sms, cudaStream_t stream) {
     switch (a.kind) {
-        case kF32: return launch_types<float, float>(a, stream);
+        case kF32: return launch_types<float, float>(a, num_sms, stream);
         case kF16:
-            return a.resid_kind == kF32 ? launch_types<__half, float>(a, stream) : launch_types<__half, __half>(a, stream);
+            return a.resid_kind == kF32 ? launch_types<__half, float>(a, num_sms, stream)
+                                        : launch_types<__half, __half>(a, num_sms, stream);
         case kBF16:
-            return a.resid_kind == kF32 ? launch_types<__nv_bfloat16, float>(a, stream)
-                                        : launch_types<__nv_bfloat16, __nv_bfloat16>(a, stream);
+            return a.resid_kind == kF32 ? launch_types<__nv_bfloat16, float>(a, num_sms, stream)
+                                        : launch_types<__nv_bfloat16, __nv_bfloat16>(a, num_sms, stream);
     }
     return cudaErrorInvalidValue;
 }

@@ -262,10 +262,12 @@ struct NormResidualArgs {
     int64_t u_stride;
     float* u_scale;           // u_eight: [ceil(dim/128)][u_scale_stride]
     int64_t u_scale_stride;
-    int vec;                  // every row starts at a 16-byte boundary
+    int vec;                  // every row starts at a 16-byte boundary, dim % 8 == 0
+    int* status;
 };
 constexpr int kNormMaxDim = 16384;
-cudaError_t launch_norm_residual(const NormResidualArgs& a, cudaStream_t stream);
+cudaError_t launch_norm_residual(const NormResidualArgs& a, int num_sms, cudaStream_t stream);
+cudaError_t norm_prepare();
 
 // Rotary positions on the heads of one or two tensors of the same tokens.
 struct RotaryPart {

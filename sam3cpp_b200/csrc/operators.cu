@@ -208,7 +208,10 @@ int s3t_norm_residual(int device, const s3t_norm_args* p, void* stream) {
         a.u = p->u.data; a.u_stride = p->u.stride;
         a.u_scale = p->u.scale; a.u_scale_stride = p->u.scale_stride;
         a.vec = vec;
-        return run_on(op, device, [&](const DeviceView&) { return launch_norm_residual(a, static_cast<cudaStream_t>(stream)); });
+        return run_on(op, device, [&](const DeviceView& dev) {
+            a.status = dev.status;
+            return launch_norm_residual(a, dev.num_sms, static_cast<cudaStream_t>(stream));
+        });
     } S3T_CATCH("norm_residual")
 }
 

@@ -160,6 +160,15 @@ S3T_DEV void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x
         : "memory");
 }
 
+// Untiled bulk copy global -> shared (both 16-byte aligned, a multiple of 16
+// bytes), counted on an mbarrier of this CTA.
+S3T_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
 // ------------------------------------------------- CTA pair (cluster of 2) ---
 
 S3T_DEV uint32_t cluster_ctarank() {

@@ -20,6 +20,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kTableEntries = 2048;   // cos/sin pairs a CTA holds (16 KB)
 constexpr int kMaxTokens = 64;        // tokens a CTA takes
+constexpr int kAhead = 4;             // heads a thread has in flight
 
 // Consecutive elements of one 16-byte access.
 template <typename T>
@@ -74,42 +75,66 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a, in
     }
     if (threadIdx.x < tokens) position[threadIdx.x] = a.positions[t0 + threadIdx.x];
     __syncthreads();
+    // A head's slots lie on consecutive threads, and a thread keeps its slot;
+    // kAhead heads are on their way at a time.
     const int heads = a.part[0].heads + a.part[1].heads;
-    const int per_token = heads * slots;
-    for (int i = threadIdx.x; i < tokens * per_token; i += kThreads) {
-        const int t = i / per_token, in_token = i - t * per_token;
-        if (position[t] < 0) continue;
-        int h = in_token / slots;
-        const int slot = in_token - h * slots;
-        const bool second = h >= a.part[0].heads;
-        const RotaryPart& part = a.part[second];
-        if (second) h -= a.part[0].heads;
-        const T* x = static_cast<const T*>(part.x) + (t0 + t) * part.x_token + h * part.x_head;
-        T* out = static_cast<T*>(part.out) + (t0 + t) * part.out_token + h * part.out_head;
-        if (slot >= turned) {
-            const int c = a.rot + (slot - turned) * V;
-            if (x != out) {
-                float v[V];
-                load_run<T, V>(x + c, v);
-                store_run<T, V>(out + c, v);
-            }
-        } else if constexpr (INTERLEAVED && V > 1) {
-            float v[V];
-            load_run<T, V>(x + slot * V, v);
-            const float2* cs = table + t * pairs + slot * (V / 2);
-#pragma unroll
-            for (int k = 0; k < V / 2; ++k) turn(v[2 * k], v[2 * k + 1], cs[k]);
-            store_run<T, V>(out + slot * V, v);
+    const int lanes = min(slots, kThreads), at_once = kThreads / lanes;
+    const int first = int(threadIdx.x) / lanes;
+    if (first >= at_once) return;
+    const int total = tokens * heads;
+    for (int slot = int(threadIdx.x) - first * lanes; slot < slots; slot += lanes) {
+        const bool turned_slot = slot < turned;
+        // Columns of the slot's runs, and its first entry of a token's table.
+        const bool pair_runs = turned_slot && !(INTERLEAVED && V > 1);
+        int ca, cb, entry;
+        if (!turned_slot) {
+            ca = cb = a.rot + (slot - turned) * V;
+            entry = 0;
+        } else if (INTERLEAVED) {
+            ca = V > 1 ? slot * V : 2 * slot;
+            cb = ca + 1;
+            entry = V > 1 ? slot * (V / 2) : slot;
         } else {
-            const int ca = INTERLEAVED ? 2 * slot : slot * V, cb = INTERLEAVED ? 2 * slot + 1 : ca + pairs;
-            float va[V], vb[V];
-            load_run<T, V>(x + ca, va);
-            load_run<T, V>(x + cb, vb);
-            const float2* cs = table + t * pairs + slot * V;
+            ca = slot * V;
+            cb = ca + pairs;
+            entry = slot * V;
+        }
+        for (int r0 = first; r0 < total; r0 += kAhead * at_once) {
+            T* to[kAhead];
+            float va[kAhead][V], vb[kAhead][V];
+            int token[kAhead];
 #pragma unroll
-            for (int k = 0; k < V; ++k) turn(va[k], vb[k], cs[k]);
-            store_run<T, V>(out + ca, va);
-            store_run<T, V>(out + cb, vb);
+            for (int k = 0; k < kAhead; ++k) {
+                const int r = r0 + k * at_once;
+                const int t = r < total ? r / heads : 0;
+                int h = r - t * heads;
+                token[k] = t;
+                to[k] = nullptr;
+                if (r >= total || position[t] < 0) continue;
+                const bool second = h >= a.part[0].heads;
+                const RotaryPart& part = a.part[second];
+                if (second) h -= a.part[0].heads;
+                const T* x = static_cast<const T*>(part.x) + (t0 + t) * part.x_token + h * part.x_head;
+                T* out = static_cast<T*>(part.out) + (t0 + t) * part.out_token + h * part.out_head;
+                if (!turned_slot && x == out) continue;
+                to[k] = out;
+                load_run<T, V>(x + ca, va[k]);
+                if (pair_runs) load_run<T, V>(x + cb, vb[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                if (!to[k]) continue;
+                const float2* cs = table + token[k] * pairs + entry;
+                if (pair_runs) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) turn(va[k][i], vb[k][i], cs[i]);
+                    store_run<T, V>(to[k] + cb, vb[k]);
+                } else if (turned_slot) {
+#pragma unroll
+                    for (int i = 0; i + 1 < V; i += 2) turn(va[k][i], va[k][i + 1], cs[i / 2]);
+                }
+                store_run<T, V>(to[k] + ca, va[k]);
+            }
         }
     }
 }

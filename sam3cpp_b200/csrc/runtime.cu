@@ -114,6 +114,7 @@ int device_state(int device, DeviceState** out) {
         S3T_CUDA(mha32_prepare());
         S3T_CUDA(neck_prepare());
         S3T_CUDA(fp8_prepare());
+        S3T_CUDA(norm_prepare());
         const std::vector<float> rl = rope_table(1.0f, kWindow);
         const std::vector<float> rg = rope_table(float(kWindow) / float(kGrid), kGrid);
         S3T_CUDA(cudaMalloc(&d.rope_local, rl.size() * 4));
