@@ -29,6 +29,7 @@ namespace {
 constexpr int kTileM = 128;
 constexpr uint32_t kStageRow = kScaleBlock;                    // bytes of a K group of one row
 constexpr uint32_t kHalfBytes = kTileM * kStageRow;            // 128 rows of a group
+constexpr int kMaxSplits = 8;                                  // CTAs that share a tile's groups
 
 template <int OUT>
 struct OutType;
@@ -258,11 +259,18 @@ __global__ void __launch_bounds__(192)
         for (int j = BN * rank / splits + warp; j < j1; j += Cfg::THREADS / 32) {
             const int m = m0 + j, n = n0 + lane * 4;
             if (m >= args.M) break;
-            float v[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int q = 0; q < splits; ++q) {
-                const float4 p = ld_cluster_f4(mapa_shared(red, q) + (j * kTileM + lane * 4) * 4);
-                v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w;
-            }
+            // All the cluster's parts at once (one after the other is a remote
+            // latency each), added in the order of the ranks.
+            float4 part[kMaxSplits];
+#pragma unroll
+            for (int q = 0; q < kMaxSplits; ++q)
+                if (q < splits) part[q] = ld_cluster_f4(mapa_shared(red, q) + (j * kTileM + lane * 4) * 4);
+            float v[4] = {part[0].x, part[0].y, part[0].z, part[0].w};
+#pragma unroll
+            for (int q = 1; q < kMaxSplits; ++q)
+                if (q < splits) {
+                    v[0] += part[q].x; v[1] += part[q].y; v[2] += part[q].z; v[3] += part[q].w;
+                }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (args.bias && n + i < args.N) v[i] += __ldg(args.bias + n + i);
@@ -318,7 +326,7 @@ cudaError_t launch_tile(const GemmFp8Args& a, int num_sms, cudaStream_t stream) 
     if (tiles > (1 << 27)) return cudaErrorInvalidValue;
     const int groups = (a.K + kScaleBlock - 1) / kScaleBlock;
     int splits = 1;
-    while (splits < 8 && 2 * splits <= groups && tiles * 2 * splits <= 2 * num_sms) splits *= 2;
+    while (splits < kMaxSplits && 2 * splits <= groups && tiles * 2 * splits <= 2 * num_sms) splits *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(uint32_t(tiles) * splits);
     cfg.blockDim = dim3(Cfg::THREADS);
