@@ -14,7 +14,7 @@
 // one number per row and group.
 //
 // gemm_fp8_tile_kernel: for few rows, with the operands swapped: 128 rows of w
-// are the UMMA's M and 16 to 128 rows of x its N, so one token costs one pass
+// are the UMMA's M and 16 to 64 rows of x its N, so one token costs one pass
 // over the weights at full load width.  The groups are split over the CTAs of a
 // cluster, which add their fp32 tiles through distributed shared memory in a
 // fixed order: no workspace, no atomics, the same result every time.
@@ -42,14 +42,21 @@ struct OutType<kBF16> { using T = __nv_bfloat16; };
 template <>
 struct OutType<kE4M3> { using T = uint8_t; };
 
+// Four accumulator columns times their factors, added to two sums.
+S3T_DEV void add4(const uint32_t* r, const float* factors, float2& a, float2& b) {
+    const float4 f = *reinterpret_cast<const float4*>(factors);
+    a = __ffma2_rn(make_float2(__uint_as_float(r[0]), __uint_as_float(r[1])), make_float2(f.x, f.y), a);
+    b = __ffma2_rn(make_float2(__uint_as_float(r[2]), __uint_as_float(r[3])), make_float2(f.z, f.w), b);
+}
+
 S3T_DEV float2 packed_fma(float a0, float a1, float2 s, float2 c) { return __ffma2_rn(make_float2(a0, a1), s, c); }
 
 // ------------------------------------------------------------- few rows ---
 
 template <int BN>
 struct TileCfg {
-    static constexpr int STAGES = BN <= 32 ? 5 : BN == 64 ? 4 : 3;
-    static constexpr int ACCS = BN == 128 ? 2 : 4;             // accumulators in flight
+    static constexpr int STAGES = BN <= 32 ? 5 : 4;
+    static constexpr int ACCS = 4;                             // accumulators in flight
     static constexpr uint32_t TMEM_COLS = ACCS * BN;
     static constexpr uint32_t X_BYTES = BN * kStageRow;
     static constexpr uint32_t STAGE_BYTES = kHalfBytes + X_BYTES;
@@ -95,10 +102,28 @@ __global__ void __launch_bounds__(192)
     const int groups = (args.K + kScaleBlock - 1) / kScaleBlock;
     const int g0 = int(int64_t(groups) * rank / splits), g1 = int(int64_t(groups) * (rank + 1) / splits);
 
+    // The producer makes the barriers and asks for the first stages before the
+    // other warps are ready: a call of one token is all latency.
+    int s = 0, g = g0;
+    uint32_t ph = 0, armed = 0, armed_parity = 0;
+    auto load = [&]() {
+        mbar_arrive_expect_tx(full + s, Cfg::STAGE_BYTES);
+        armed |= 1u << s;
+        armed_parity = (armed_parity & ~(1u << s)) | (ph << s);
+        tma_load_2d(sW + s * kHalfBytes, &tmW, full + s, g * kScaleBlock, n0);
+        tma_load_2d(sX + s * Cfg::X_BYTES, &tmX, full + s, g * kScaleBlock, m0);
+        ++g;
+        if (++s == Cfg::STAGES) {
+            s = 0;
+            ph ^= 1;
+        }
+    };
     if (threadIdx.x == 0) {
-        for (int s = 0; s < Cfg::STAGES; ++s) {
-            mbar_init(full + s, 1);
-            mbar_init(empty + s, 1);
+        tma_prefetch_desc(&tmW);
+        tma_prefetch_desc(&tmX);
+        for (int i = 0; i < Cfg::STAGES; ++i) {
+            mbar_init(full + i, 1);
+            mbar_init(empty + i, 1);
         }
         for (int i = 0; i < Cfg::ACCS; ++i) {
             mbar_init(tfull + i, 1);
@@ -107,6 +132,7 @@ __global__ void __launch_bounds__(192)
         mbar_init(drain, 1);
         *abort_flag = 0;
         fence_barrier_init();
+        while (g < g1 && g - g0 < Cfg::STAGES) load();
     }
     if (warp == 1) {
         tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
@@ -119,23 +145,13 @@ __global__ void __launch_bounds__(192)
 
     if (warp == 0) {
         if (lane == 0) {
-            int s = 0;
-            uint32_t ph = 0, armed = 0, armed_parity = 0;
             bool ok = true;
-            for (int g = g0; g < g1; ++g) {
+            while (g < g1) {
                 if (!mbar_wait(empty + s, ph ^ 1, args.status, kErrTimeoutProducer, abort_flag)) {
                     ok = false;
                     break;
                 }
-                mbar_arrive_expect_tx(full + s, Cfg::STAGE_BYTES);
-                armed |= 1u << s;
-                armed_parity = (armed_parity & ~(1u << s)) | (ph << s);
-                tma_load_2d(sW + s * kHalfBytes, &tmW, full + s, g * kScaleBlock, n0);
-                tma_load_2d(sX + s * Cfg::X_BYTES, &tmX, full + s, g * kScaleBlock, m0);
-                if (++s == Cfg::STAGES) {
-                    s = 0;
-                    ph ^= 1;
-                }
+                load();
             }
             if (!ok) {
                 for (int i = 0; i < Cfg::STAGES; ++i)
@@ -185,15 +201,22 @@ __global__ void __launch_bounds__(192)
         // load into a register would stall the warp at its first use.
         float* raw = scales + (warp - 2) * Cfg::SCALE_WORDS + lane;
         float* products = scales + (warp - 2) * Cfg::SCALE_WORDS + Cfg::SCALE_SLOTS * 32 * (PER_LANE + 1);
-        const int nb = n0 / kScaleBlock;
+        const float* ahead_w = args.ws + int64_t(g0) * args.ws_stride + n0 / kScaleBlock;
+        const float* ahead_x = args.xs + int64_t(g0) * args.xs_stride + (m0 + lane < args.M ? m0 + lane : 0);
         auto fetch = [&](int g) {
             float* slot = raw + ((g - g0) % Cfg::SCALE_SLOTS) * 32 * (PER_LANE + 1);
-            cp_async4(slot, g < g1 ? args.ws + int64_t(g) * args.ws_stride + nb : args.ws, g < g1);
+            if (g < g1) {
+                cp_async4(slot, ahead_w, true);
 #pragma unroll
-            for (int i = 0; i < PER_LANE; ++i) {
-                const int j = lane + 32 * i, m = m0 + j;
-                const bool take = g < g1 && j < BN && m < args.M;
-                cp_async4(slot + 32 * (i + 1), take ? args.xs + int64_t(g) * args.xs_stride + m : args.xs, take);
+                for (int i = 0; i < PER_LANE; ++i) {
+                    const int j = lane + 32 * i;
+                    const bool take = j < BN && m0 + j < args.M;
+                    cp_async4(slot + 32 * (i + 1), ahead_x + (take ? 32 * i : 0), take);
+                }
+                if (g + 1 < g1) {
+                    ahead_w += args.ws_stride;
+                    ahead_x += args.xs_stride;
+                }
             }
             cp_async_commit();
         };
@@ -220,19 +243,16 @@ __global__ void __launch_bounds__(192)
                 tmem_ld16(t, r);
                 tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    sum[c] = packed_fma(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]),
-                                        *reinterpret_cast<const float2*>(sc + 2 * c), sum[c]);
+                for (int c = 0; c < 4; ++c) add4(r + 4 * c, sc + 4 * c, sum[2 * c], sum[2 * c + 1]);
             } else {
 #pragma unroll
                 for (int b = 0; b < BN / 32; ++b) {
                     uint32_t r[32];
                     tmem_ld32(t + 32 * b, r);
-                    tmem_wait_ld();
+                    tmem_wait_ld(r);
 #pragma unroll
-                    for (int c = 0; c < 16; ++c)
-                        sum[16 * b + c] = packed_fma(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]),
-                                                     *reinterpret_cast<const float2*>(sc + 32 * b + 2 * c), sum[16 * b + c]);
+                    for (int c = 0; c < 8; ++c)
+                        add4(r + 4 * c, sc + 32 * b + 4 * c, sum[16 * b + 2 * c], sum[16 * b + 2 * c + 1]);
                 }
             }
             tc_fence_before();
@@ -315,6 +335,24 @@ __global__ void __launch_bounds__(192)
     }
 }
 
+int groups_of(int K) { return K / kScaleBlock + (K % kScaleBlock != 0); }
+
+// CTAs that share a tile's groups: as many as give every SM one CTA, or two
+// while each has eight groups and more.  (1 x 4736 x 1024: 5.5 us with 148
+// CTAs, 8.1 us with 296 of one group; 1 x 8192 x 8192: 12.8 us with 256 CTAs
+// of 16 groups, 16.7 us with 128 of 32.)
+int tile_splits(int64_t tiles, int groups, int num_sms) {
+    int splits = 1;
+    while (2 * splits <= kMaxSplits && 2 * splits <= groups &&
+           tiles * 2 * splits <= (groups >= 16 * splits ? 2 * num_sms : num_sms))
+        splits *= 2;
+    return splits;
+}
+
+int64_t tiles_of(int M, int N, int bm, int bn) {
+    return (int64_t(M) + bm - 1) / bm * ((int64_t(N) + bn - 1) / bn);
+}
+
 template <int BN, int OUT>
 cudaError_t launch_tile(const GemmFp8Args& a, int num_sms, cudaStream_t stream) {
     using Cfg = TileCfg<BN>;
@@ -322,11 +360,9 @@ cudaError_t launch_tile(const GemmFp8Args& a, int num_sms, cudaStream_t stream) 
     if (!make_tmap_rows(&tw, a.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.K, a.N, a.w_stride, kStageRow, kTileM) ||
         !make_tmap_rows(&tx, a.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.K, a.M, a.x_stride, kStageRow, BN))
         return cudaErrorInvalidValue;
-    const int64_t tiles = (int64_t(a.N) + kTileM - 1) / kTileM * ((int64_t(a.M) + BN - 1) / BN);
+    const int64_t tiles = tiles_of(a.M, a.N, BN, kTileM);
     if (tiles > (1 << 27)) return cudaErrorInvalidValue;
-    const int groups = (a.K + kScaleBlock - 1) / kScaleBlock;
-    int splits = 1;
-    while (splits < kMaxSplits && 2 * splits <= groups && tiles * 2 * splits <= 2 * num_sms) splits *= 2;
+    const int splits = tile_splits(tiles, groups_of(a.K), num_sms);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(uint32_t(tiles) * splits);
     cfg.blockDim = dim3(Cfg::THREADS);
@@ -720,14 +756,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
                     if (lane == 0) tma_store_2d(&tmY, buf, n, row0);
                 } else {
                     __syncwarp();
-                    for (int rr = 0; rr < 32 && row0 + rr < args.M; ++rr) {
-                        T* y = static_cast<T*>(args.y) + int64_t(row0 + rr) * args.y_stride;
+#pragma unroll 8
+                    for (int rr = 0; rr < 32; ++rr) {
+                        T* y = static_cast<T*>(args.y) + int64_t(row0 + rr) * args.y_stride + n;
 #pragma unroll
                         for (int k = 0; k < CHUNK_COLS / 32; ++k) {
                             const int col = lane + 32 * k, byte = col * ELEM;
-                            if (n + col < args.N)
-                                y[n + col] = *reinterpret_cast<const T*>(buf + rr * Cfg::OUT_ROW +
-                                                                         (((byte >> 4) ^ (rr & 7)) << 4) + (byte & 15));
+                            const T v = *reinterpret_cast<const T*>(buf + rr * Cfg::OUT_ROW +
+                                                                    (((byte >> 4) ^ (rr & 7)) << 4) + (byte & 15));
+                            if (row0 + rr < args.M && n + col < args.N) y[col] = v;
                         }
                     }
                     __syncwarp();
@@ -769,12 +806,22 @@ cudaError_t launch_pair(const GemmFp8Args& a, int num_sms, cudaStream_t stream) 
     return cudaGetLastError();
 }
 
+// Up to 32 rows the narrow tiles.  Above, what takes less by the two kernels'
+// measured steps: a 128 x 64 tile's CTA takes about 0.6 us a group after 5.5 us
+// of set-up and joining, a 256 x 256 tile's pair 0.42 us after 6.5 us.  (us,
+// tiles against pairs: 201 x 1024 x 4736 11.2 / 22.5, 400 x 1024 x 1024 8.5 /
+// 9.9, 201 x 4736 x 1024 11.5 / 9.6, 1600 x 1024 x 4736 36.9 / 22.9, 201 x 8192
+// x 8192 58 / 35.)
 template <int OUT>
 cudaError_t launch_out(const GemmFp8Args& a, int num_sms, cudaStream_t stream) {
     if (a.M <= 16) return launch_tile<16, OUT>(a, num_sms, stream);
     if (a.M <= 32) return launch_tile<32, OUT>(a, num_sms, stream);
-    if (a.M <= 64) return launch_tile<64, OUT>(a, num_sms, stream);
-    if (a.M <= 2048) return launch_tile<128, OUT>(a, num_sms, stream);
+    const int64_t groups = groups_of(a.K);
+    const int64_t tiles = tiles_of(a.M, a.N, 64, kTileM), pairs = tiles_of(a.M, a.N, 2 * kTileM, PairCfg8::BN);
+    const int splits = tile_splits(tiles, int(groups), num_sms);
+    const int64_t rounds = (tiles * splits + num_sms - 1) / num_sms, waves = (pairs + num_sms / 2 - 1) / (num_sms / 2);
+    const int64_t tile_time = 550 + 60 * rounds * ((groups + splits - 1) / splits), pair_time = 650 + 42 * waves * groups;
+    if (tile_time <= pair_time) return launch_tile<64, OUT>(a, num_sms, stream);
     return launch_pair<OUT>(a, num_sms, stream);
 }
 
@@ -790,7 +837,6 @@ cudaError_t prepare_out() {
     if ((e = prepare_tile<16, OUT>()) != cudaSuccess) return e;
     if ((e = prepare_tile<32, OUT>()) != cudaSuccess) return e;
     if ((e = prepare_tile<64, OUT>()) != cudaSuccess) return e;
-    if ((e = prepare_tile<128, OUT>()) != cudaSuccess) return e;
     return cudaFuncSetAttribute(gemm_fp8_pair_kernel<OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 int(PairCfg8::SMEM));
 }
