@@ -20,6 +20,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kTableEntries = 2048;   // cos/sin pairs a CTA holds (16 KB)
 constexpr int kMaxTokens = 64;        // tokens a CTA takes
+constexpr int kRows = 512;            // heads whose places a CTA holds at a time
 
 // Consecutive elements of one 16-byte access.
 template <typename T>
@@ -62,7 +63,7 @@ S3T_DEV void turn(float& a, float& b, float2 cs) {
 // columns where V > 1) and then the slots of V columns that pass through.  A
 // head's slots lie on consecutive threads and a thread keeps its slot; its
 // first head is on its way while the CTA makes the table.  65536 tokens of
-// 20 heads of 128, 16-bit: 116 us in halves (5.8 TB/s), 126 us interleaved
+// 20 heads of 128, 16-bit: 117 us in halves (5.7 TB/s), 123 us interleaved
 // with 96 columns turned; two or four heads in flight a thread took 124 and
 // 164 us, since fewer CTAs fit an SM.
 template <typename T, int V, bool INTERLEAVED>
@@ -70,6 +71,8 @@ __global__ void __launch_bounds__(kThreads, INTERLEAVED ? 8 : 6)
     rotary_kernel(const RotaryArgs a, int tokens_per_cta, int turned, int slots) {
     __shared__ float2 table[kTableEntries];
     __shared__ int64_t position[kMaxTokens];
+    __shared__ ulonglong2 row_at[kRows];      // x and out of a head
+    __shared__ short row_token[kRows];
     const int64_t t0 = int64_t(blockIdx.x) * tokens_per_cta;
     const int tokens = int(min(int64_t(tokens_per_cta), a.tokens - t0));
     const int pairs = a.rot / 2;
@@ -97,27 +100,39 @@ __global__ void __launch_bounds__(kThreads, INTERLEAVED ? 8 : 6)
             entry = slot * V;
         }
     };
+    // Where rows base .. of the CTA's heads are: the divisions and 64-bit
+    // products once a head, not once a slot.
+    auto places = [&](int base) {
+        for (int i = threadIdx.x; i < kRows && base + i < total; i += kThreads) {
+            const int r = base + i, t = r / heads;
+            int h = r - t * heads;
+            const bool second = h >= a.part[0].heads;
+            const RotaryPart& part = a.part[second];
+            if (second) h -= a.part[0].heads;
+            const T* x = static_cast<const T*>(part.x) + (t0 + t) * part.x_token + h * part.x_head;
+            T* out = static_cast<T*>(part.out) + (t0 + t) * part.out_token + h * part.out_head;
+            row_at[i] = make_ulonglong2(reinterpret_cast<unsigned long long>(x), reinterpret_cast<unsigned long long>(out));
+            row_token[i] = short(t);
+        }
+    };
     T* to;
-    int token;
     Run<T, V> ra, rb;
-    auto load = [&](int r) {
-        to = nullptr;
-        if (r >= total) return;
-        token = r / heads;
-        int h = r - token * heads;
-        const bool second = h >= a.part[0].heads;
-        const RotaryPart& part = a.part[second];
-        if (second) h -= a.part[0].heads;
-        const T* x = static_cast<const T*>(part.x) + (t0 + token) * part.x_token + h * part.x_head;
-        T* out = static_cast<T*>(part.out) + (t0 + token) * part.out_token + h * part.out_head;
-        if (!turned_slot && x == out) return;
-        to = out;
+    auto load = [&](int i) {   // row i of those whose places are known
+        const ulonglong2 at = row_at[i];
+        const T* x = reinterpret_cast<const T*>(at.x);
+        to = reinterpret_cast<T*>(at.y);
+        if (!turned_slot && x == to) {
+            to = nullptr;
+            return;
+        }
         load_run(x + ca, ra);
         if (pair_runs) load_run(x + cb, rb);
     };
     const bool works = first < at_once;
     place();
-    if (works) load(first);
+    places(0);
+    __syncthreads();
+    if (works && first < total) load(first);   // first < at_once <= kRows
 
     for (int i = threadIdx.x; i < tokens * pairs; i += kThreads) {
         const int t = i / pairs, p = i - t * pairs;
@@ -130,34 +145,46 @@ __global__ void __launch_bounds__(kThreads, INTERLEAVED ? 8 : 6)
     }
     if (threadIdx.x < tokens) position[threadIdx.x] = a.positions[t0 + threadIdx.x];
     __syncthreads();
-    if (!works) return;
-    while (true) {
-        for (int r = first; r < total; r += at_once) {
-            if (r != first) load(r);
-            if (!to || position[token] < 0) continue;
-            if (turned_slot) {
-                const float2* cs = table + token * pairs + entry;
-                float va[V];
-                widen(ra, va);
-                if (pair_runs) {
-                    float vb[V];
-                    widen(rb, vb);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) turn(va[i], vb[i], cs[i]);
-                    narrow(vb, rb);
-                    store_run(to + cb, rb);
-                } else {
-#pragma unroll
-                    for (int i = 0; i + 1 < V; i += 2) turn(va[i], va[i + 1], cs[i / 2]);
-                }
-                narrow(va, ra);
+    for (int base = 0;;) {
+        const int here = min(kRows, total - base);
+        for (int s0 = 0; works && s0 + slot < slots; s0 += lanes) {   // again where a head has more slots than threads
+            if (s0) {
+                slot += s0;
+                place();
             }
-            store_run(to + ca, ra);
+            for (int i = first; i < here; i += at_once) {
+                if (base || s0 || i != first) load(i);
+                const int token = row_token[i];
+                if (!to || position[token] < 0) continue;
+                if (turned_slot) {
+                    const float2* cs = table + token * pairs + entry;
+                    float va[V];
+                    widen(ra, va);
+                    if (pair_runs) {
+                        float vb[V];
+                        widen(rb, vb);
+#pragma unroll
+                        for (int k = 0; k < V; ++k) turn(va[k], vb[k], cs[k]);
+                        narrow(vb, rb);
+                        store_run(to + cb, rb);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k + 1 < V; k += 2) turn(va[k], va[k + 1], cs[k / 2]);
+                    }
+                    narrow(va, ra);
+                }
+                store_run(to + ca, ra);
+            }
+            if (s0) {
+                slot -= s0;
+                place();
+            }
         }
-        slot += lanes;   // more slots than threads
-        if (slot >= slots) break;
-        place();
-        load(first);
+        base += kRows;
+        if (base >= total) break;
+        __syncthreads();
+        places(base);
+        __syncthreads();
     }
 }
 
