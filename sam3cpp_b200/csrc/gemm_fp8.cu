@@ -297,7 +297,11 @@ __global__ void __launch_bounds__(192)
             }
             if (args.gelu) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = gelu_erf_as(v[i]);
+                for (int i = 0; i < 2; ++i) {
+                    const float2 t = gelu_erf_poly2(make_float2(v[2 * i], v[2 * i + 1]));
+                    v[2 * i] = t.x;
+                    v[2 * i + 1] = t.y;
+                }
             }
             T* row = static_cast<T*>(args.y) + int64_t(m) * args.y_stride;
             const bool whole = args.vec && n + 4 <= args.N;
@@ -703,7 +707,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
             }
             if (args.gelu) {
 #pragma unroll
-                for (int i = 0; i < Cfg::WARP_COLS / 2; ++i) sum[i] = gelu_erf_as2(sum[i]);
+                for (int i = 0; i < Cfg::WARP_COLS / 2; ++i) sum[i] = gelu_erf_poly2(sum[i]);
             }
             // Each lane writes 128 bytes of its row at a time to a swizzled stage,
             // and one TMA store per warp takes the 32 rows while the next tile is
