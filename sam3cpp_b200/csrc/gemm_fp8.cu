@@ -619,7 +619,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
         const uint32_t lanes = uint32_t(quarter * 32) << 16;
         uint8_t* stage = sOut + (warp - 4) * Cfg::OUT_BUFS * Cfg::OUT_BUF;
         float* my_bias = biases + (warp - 4) * Cfg::WARP_COLS;
-        const float* my_factor = factors + half * kTileM + quarter * 32 + lane;
+        const uint32_t my_factor = smem_u32(factors + half * kTileM + quarter * 32 + lane);
         int it = 0, out = 0, s = 0;   // groups promoted, the next buffer of y, the group's stage
         uint32_t ph = 0;
         bool ok = true;
@@ -665,7 +665,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
             if (!ok) break;
             tmem_ld32(t, r[0]);
             tmem_ld32(t + 32, r[1]);
-            f = my_factor[(it % Cfg::FACTOR_SLOTS) * Cfg::FACTOR_WORDS];
+            f = ld_shared_f(my_factor + (it % Cfg::FACTOR_SLOTS) * Cfg::FACTOR_WORDS * 4);
 #pragma unroll 1
             for (int g = 0; g < groups; ++g) {
                 tmem_wait_ld(r[0]);
@@ -688,7 +688,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
                 ok = next_group();
                 if (!ok) break;
                 tmem_ld32(t, r[0]);
-                const float f_next = my_factor[(it % Cfg::FACTOR_SLOTS) * Cfg::FACTOR_WORDS];
+                const float f_next = ld_shared_f(my_factor + (it % Cfg::FACTOR_SLOTS) * Cfg::FACTOR_WORDS * 4);
                 add(r[1], 3);
                 tmem_ld32(t + 32, r[1]);
                 f = f_next;
@@ -699,10 +699,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
                 cp_async_wait<0>();   // issued a tile ago
                 __syncwarp();
 #pragma unroll
-                for (int i = 0; i < Cfg::WARP_COLS / 4; ++i) {
-                    const float4 b = *reinterpret_cast<const float4*>(my_bias + 4 * i);
-                    sum[2 * i] = __fadd2_rn(sum[2 * i], make_float2(b.x, b.y));
-                    sum[2 * i + 1] = __fadd2_rn(sum[2 * i + 1], make_float2(b.z, b.w));
+                for (int i = 0; i < Cfg::WARP_COLS / 4; i += 8) {
+                    float4 b[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) b[k] = ld_shared_f4(smem_u32(my_bias) + 16 * (i + k));
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        sum[2 * (i + k)] = __fadd2_rn(sum[2 * (i + k)], make_float2(b[k].x, b[k].y));
+                        sum[2 * (i + k) + 1] = __fadd2_rn(sum[2 * (i + k) + 1], make_float2(b[k].z, b[k].w));
+                    }
                 }
             }
             if (args.gelu) {
@@ -721,10 +726,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
             constexpr int CHUNK_COLS = int(Cfg::OUT_ROW) / ELEM;
             BlockScale bs{0.f, 0.f};
             if constexpr (OUT == kE4M3) {
-                uint32_t a = 0;
+                float a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < Cfg::WARP_COLS / 2; ++i) a = max(a, max(abs_bits(sum[i].x), abs_bits(sum[i].y)));
-                bs = block_scale(a);
+                for (int i = 0; i < Cfg::WARP_COLS / 2; ++i) a[i & 3] = absmax3_nan(a[i & 3], sum[i].x, sum[i].y);
+                bs = block_scale(__float_as_uint(absmax3_nan(absmax3_nan(a[0], a[1], a[2]), a[3], a[3])) & 0x7fffffffu);
                 if (row0 + lane < args.M) args.ys[int64_t(n0 / kScaleBlock) * args.ys_stride + row0 + lane] = bs.scale;
             }
 #pragma unroll
@@ -735,7 +740,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
                 out = out + 1 == Cfg::OUT_BUFS ? 0 : out + 1;
                 if (lane == 0) bulk_wait_group_read<Cfg::OUT_BUFS - 1>();   // the chunk that was in buf has left it
                 __syncwarp();
-                uint8_t* rowp = buf + lane * Cfg::OUT_ROW;
+                const uint32_t rowp = smem_u32(buf + lane * Cfg::OUT_ROW);
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     uint32_t w[4];
@@ -752,7 +757,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
                             w[i] = pack2(v.x, v.y, T());
                         }
                     }
-                    *reinterpret_cast<uint4*>(rowp + ((q ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    st_shared_u4(rowp + ((q ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
                 }
                 if (args.vec && (n + CHUNK_COLS <= args.N || int64_t(args.N) * ELEM % 16 == 0)) {
                     fence_proxy_async_smem();

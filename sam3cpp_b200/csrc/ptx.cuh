@@ -264,6 +264,25 @@ S3T_DEV void fence_proxy_async_smem() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// ---------------------------------------------- shared memory by address ---
+// For pointers that went through integer alignment, which the compiler would
+// reach by slower generic accesses.
+S3T_DEV float4 ld_shared_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+S3T_DEV float ld_shared_f(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+S3T_DEV void st_shared_u4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
 // -------------------------------------------------------- register split ---
 // Every warp of a warpgroup (four warps) gives up or takes registers per
 // thread; the warpgroups' shares must add up to no more than the launch's.
@@ -484,6 +503,13 @@ S3T_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
 S3T_DEV float fmax3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// Largest magnitude of three, NaN if one is NaN.
+S3T_DEV float absmax3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 
