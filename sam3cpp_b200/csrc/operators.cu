@@ -29,6 +29,9 @@ int element_kind(int type) {
     return -1;
 }
 
+// Keeps a size rounded up to whole tiles inside 32 bits.
+constexpr int kMost = 1 << 30;
+
 int element_bytes(int kind) { return kind == kF32 ? 4 : kind == kE4M3 ? 1 : 2; }
 
 bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % uintptr_t(bytes) == 0; }
@@ -106,6 +109,7 @@ int s3t_gemm_fp8(int device, const s3t_matrix* x, const s3t_matrix* w, const flo
         const int kind = element_kind(y_type);
         if (kind < 0) return refuse(op, "y must be F32, F16, BF16 or E4M3");
         if (M < 0 || N < 0 || K < 1) return refuse(op, "needs M >= 0, N >= 0 and K >= 1");
+        if (M > kMost || N > kMost || K > kMost) return refuse(op, "M, N and K must be at most 2^30");
         if (act != 0 && act != 1) return refuse(op, "act must be 0 (none) or 1 (GELU)");
         if (const char* why = bad_eight(x, K, M)) return refuse(op, std::string("x: ") + why);
         if (const char* why = bad_eight(w, K, blocks(N))) return refuse(op, std::string("w: ") + why);

@@ -60,6 +60,7 @@ GEMM = dict(x=eight(), w=eight(), bias=None, m=5, n=200, k=200, act=0, y_type=s3
     (dict(m=-1), "M >= 0"),
     (dict(n=-1), "N >= 0"),
     (dict(k=0), "K >= 1"),
+    (dict(m=(1 << 30) + 1, x=eight(scale_stride=1 << 31)), "2\\^30"),
     (dict(act=2), "act"),
     (dict(y_type=8), "y must be"),
     (dict(x=None), "x: "),

@@ -211,7 +211,7 @@ def test_product_gelu(torch, m, out):
     check_product(torch, x, w, bias, True, out, call_product(torch, x, w, bias, True, out))
 
 
-LARGE = [(2048, 1024, 1024), (2500, 4736, 1024), (5184, 1000, 4736), (4097, 129, 100), (3000, 257, 4000)]
+LARGE = [(2048, 1024, 1024), (2500, 4736, 1024), (5184, 1000, 4736), (4097, 129, 100), (20000, 512, 100), (3000, 257, 4000)]
 
 
 @pytest.mark.parametrize("m, n, k", LARGE)
@@ -490,6 +490,70 @@ def test_rotary_offsets_past_32_bits(torch):
     for t in range(tokens):
         got = cache[t * stride: t * stride + dim].double()
         assert ((got - want[t, 0]).abs() <= e[t, 0] + want[t, 0].abs() * 2.0 ** -11 + 2.0 ** -25).all()
+
+
+def test_quantize_and_product_past_32_bits(torch):
+    """Rows of x, q and y that lie more than 2^32 elements apart, for both product kernels."""
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 50 GB of free device memory")
+    g = torch.Generator("cuda").manual_seed(2)
+    for m, n, k, stride in ((3, 130, 200, (1 << 31) + 16), (161, 4736, 1024, (1 << 26) + 16)):
+        w = random_eight(torch, g, n, k, 128)
+        w.scale[: w.groups, : w.blocks] *= 1e-3
+        x = torch.randn(m, k, generator=g, device="cuda").half()
+        q = torch.empty((m - 1) * stride + k, device="cuda", dtype=torch.uint8)
+        scale = torch.empty(up(k, 128) // 128, m, device="cuda")
+        s3t.quantize_fp8(0, s3t.TYPE_F16, x.data_ptr(), m, k, k, 1, s3t.Matrix(q.data_ptr(), stride, scale.data_ptr(), m))
+        codes, want_scale = quantized(torch, x.float(), 1)
+        rows = torch.stack([q[i * stride: i * stride + k] for i in range(m)]).view(torch.float8_e4m3fn)
+        assert torch.equal(rows.float(), codes.float()) and torch.equal(scale, want_scale)
+        y = torch.empty((m - 1) * stride + n, device="cuda", dtype=torch.float16)
+        xm = s3t.Matrix(q.data_ptr(), stride, scale.data_ptr(), m)
+        s3t.gemm_fp8(0, xm, w.matrix, None, m, n, k, 0, s3t.TYPE_F16, s3t.Matrix(y.data_ptr(), stride))
+        near = torch.empty(m, n, device="cuda", dtype=torch.float16)
+        s3t.gemm_fp8(0, xm, w.matrix, None, m, n, k, 0, s3t.TYPE_F16, s3t.Matrix(near.data_ptr(), n))
+        assert torch.equal(torch.stack([y[i * stride: i * stride + n] for i in range(m)]), near)
+        xv = rows.double() * scale.t().double().repeat_interleave(128, 1)[:, :k]
+        want, mag = xv @ w.values(torch).t(), xv.abs() @ w.values(torch).abs().t()
+        e = mag * (128 + up(k, 128) // 128 + 8) * 2 * U
+        assert ((near.double() - want).abs() <= e + (want.abs() + e) * 2.0 ** -11 + 2.0 ** -25).all()
+        del q, y
+
+
+def test_calls_from_two_threads(torch):
+    """Two host threads, a stream each, every operator: the same results as one after the other."""
+    import threading
+    dim, rows = 512, 300
+    g = torch.Generator("cuda").manual_seed(4)
+    w = random_eight(torch, g, 384, dim, 128)
+
+    def work(seed, stream, out):
+        gg = torch.Generator("cuda").manual_seed(seed)
+        x = torch.randn(rows, dim, generator=gg, device="cuda")
+        u = Eight(torch, rows, dim)
+        y = torch.empty(rows, 384, device="cuda", dtype=torch.float16)
+        q8 = Eight(torch, rows, 384)
+        torch.cuda.synchronize()
+        st = stream.cuda_stream
+        for _ in range(20):
+            s3t.norm_residual(0, s3t.NormArgs(rows=rows, dim=dim, type=1, resid_type=0, u_type=s3t.TYPE_E4M3, eps=1e-6,
+                                              resid_scale=1.0, x=x.data_ptr(), x_stride=dim, u=u.matrix), st)
+            s3t.gemm_fp8(0, u.matrix, w.matrix, None, rows, 384, dim, 1, s3t.TYPE_F16, s3t.Matrix(y.data_ptr(), 384), st)
+            s3t.quantize_fp8(0, s3t.TYPE_F16, y.data_ptr(), rows, 384, 384, 1, q8.matrix, st)
+        stream.synchronize()
+        out[seed] = (y.clone(), q8.q.clone(), q8.scale.clone())
+
+    alone, together = {}, {}
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for seed in (1, 2):
+        work(seed, streams[0], alone)
+    threads = [threading.Thread(target=work, args=(seed, streams[seed - 1], together)) for seed in (1, 2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for seed in (1, 2):
+        assert all(torch.equal(a, b) for a, b in zip(alone[seed], together[seed]))
 
 
 def test_small_operators_in_a_graph(torch):
