@@ -412,10 +412,10 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
     const bool whole = c0 + int(Row::COLS) <= dim;      // no column of this warp lies past dim
     bool lost = false;
     for (uint32_t it = 0; row < rows; ++it) {
-        const int slot = it & 1;
+        const int slot = int(it % kSlots);
         // A row that never came is reported; the loop goes on without waiting, so
         // that no warp of the team is left alone at a barrier.
-        lost = lost || !mbar_wait(bar + slot, (it >> 1) & 1, a.status, kErrTimeoutProducer, nullptr);
+        lost = lost || !mbar_wait(bar + slot, (it / kSlots) & 1, a.status, kErrTimeoutProducer, nullptr);
         const uint8_t* from = mine + slot * Row::BYTES;
         float2 x[CPW][4], h[CPW][4];
         auto vector = [&](int k, int j, float2(&v)[4]) { load_chunk<true>(vec + k * padded + c0 + j * kChunk, 0, kChunk, lane, v); };

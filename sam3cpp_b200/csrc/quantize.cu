@@ -48,7 +48,7 @@ S3T_DEV void load_group(const T* row, int64_t c0, int64_t cols, int lane16, Raw<
         const uint4* p = reinterpret_cast<const uint4*>(row + c0 + lane16 * 8);
 #pragma unroll
         for (int i = 0; i < int(sizeof(T)) / 2; ++i) {
-            const uint4 u = __ldcs(p + i);
+            const uint4 u = p[i];
             v.w[4 * i] = u.x; v.w[4 * i + 1] = u.y; v.w[4 * i + 2] = u.z; v.w[4 * i + 3] = u.w;
         }
         return;
@@ -112,7 +112,7 @@ S3T_DEV uint32_t float_bits(uint32_t peak) {
 // of two 16-bit rows share a word in the reduction, and each lane does one of
 // the eight divisions (a / 448 and 448 / a of four rows) of its half warp.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeArgs a, uint32_t col_blocks) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 8) quantize_rows_kernel(const QuantizeArgs a, uint32_t col_blocks) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rb = blockIdx.x / col_blocks, cb = blockIdx.x - rb * col_blocks;
     const int64_t r0 = int64_t(rb) * kRowsPerCta + warp * kRowsPerWarp;
