@@ -15,10 +15,12 @@
 //
 // Many rows (STREAM): persistent CTAs, four chunks a warp, so that a reduction
 // or a barrier is paid once for 32 columns a lane; the vectors wait in shared
-// memory and the rows ahead come there by bulk copies, two a warp.  82944 x
-// 1024, LayerNorm twice, gate, e4m3 out: 174 us, 5.4 TB/s; whole rows per warp
-// read straight into registers took 398 us (the loads' latency), one chunk a
-// warp with the next row in registers 269 us (four times the reductions).
+// memory and the next row comes there by bulk copies while the second half of
+// a row is computed.  82944 x 1024, LayerNorm twice, gate, e4m3 out: 158 us,
+// 5.9 TB/s with 16 warps an SM and one row ahead (12 warps and two rows: 174
+// us, 20 warps of fewer registers: 168 us); whole rows per warp read straight
+// into registers took 398 us (the loads' latency), one chunk a warp with the
+// next row in registers 269 us (four times the reductions).
 // Few rows: one chunk a warp up to 4096 columns, everything asked for at once,
 // for the latency of one row.
 //
@@ -35,10 +37,10 @@ namespace {
 
 constexpr int kChunk = 2 * kScaleBlock;
 constexpr int kMaxWarps = 16;          // of a team: 16 x 4 chunks hold kNormMaxDim columns
-constexpr int kSlots = 2;              // rows ahead (STREAM)
+constexpr int kSlots = 1;              // rows ahead of a warp (STREAM)
 constexpr int kStreamCpw = 4;
-constexpr int kStreamWarps = 12;
-constexpr int kStreamBytes = 220 * 1024;
+constexpr int kStreamWarps = 16;
+constexpr int kStreamBytes = 200 * 1024;
 constexpr int kVectors = 5;            // post weight and bias, branch factor, pre weight and bias
 
 // A lane's eight elements of a chunk are two quads: quad h is columns
@@ -142,7 +144,8 @@ struct Split {
     float inv_dim, inv_last;
 };
 
-// Barrier of one team's warps (named barrier 1 + team).
+// Barrier of one team's warps (named barrier 1 + team; teams of more than one
+// warp are at most eight a CTA).
 S3T_DEV void team_sync(const Split& sp) {
     asm volatile("bar.sync %0, %1;" ::"r"(sp.team + 1), "r"(sp.warps * 32) : "memory");
 }
