@@ -4,7 +4,9 @@
 //
 // Bound by HBM: each element is read once and one byte of it written.  Sixteen
 // lanes hold the 128 columns of a group, eight consecutive elements each, so
-// the group's maximum is four shuffles away and nothing is read twice.
+// the group's maximum is four shuffles away and nothing is read twice.  82944 x
+// 4736 fp16: 183 us, 6.5 TB/s (469 us with a division per lane and group and
+// the maxima in fp32: bound by its instructions; 208 us at five CTAs an SM).
 #include "elements.cuh"
 #include "fp8.cuh"
 #include "kernels.h"
@@ -24,14 +26,11 @@ struct Raw {
     uint32_t w[2 * sizeof(T)];
 };
 
+// Elements 2 i and 2 i + 1.
 template <typename T>
-S3T_DEV float element(const Raw<T>& v, int i) {
-    if constexpr (sizeof(T) == 4) {
-        return __uint_as_float(v.w[i]);
-    } else {
-        const float2 f = unpack2(v.w[i / 2], T());
-        return i & 1 ? f.y : f.x;
-    }
+S3T_DEV float2 elements(const Raw<T>& v, int i) {
+    if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(v.w[2 * i]), __uint_as_float(v.w[2 * i + 1]));
+    else return unpack2(v.w[i], T());
 }
 
 // Columns of element i of a lane's eight: consecutive where the rows are
@@ -70,10 +69,10 @@ S3T_DEV void no_group(Raw<T>& v) {
 
 template <typename T, bool VEC>
 S3T_DEV void store_group(uint8_t* row, int64_t c0, int64_t cols, int lane16, const Raw<T>& v, float inv) {
-    float f[8];
+    float2 f[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(element(v, i), inv);
-    const uint32_t lo = pack_e4m3x4(f[0], f[1], f[2], f[3]), hi = pack_e4m3x4(f[4], f[5], f[6], f[7]);
+    for (int i = 0; i < 4; ++i) f[i] = __fmul2_rn(elements(v, i), make_float2(inv, inv));
+    const uint32_t lo = pack_e4m3x4(f[0].x, f[0].y, f[1].x, f[1].y), hi = pack_e4m3x4(f[2].x, f[2].y, f[3].x, f[3].y);
     if (VEC && c0 + lane16 * 8 + 8 <= cols) {
         *reinterpret_cast<uint2*>(row + c0 + lane16 * 8) = make_uint2(lo, hi);
         return;
