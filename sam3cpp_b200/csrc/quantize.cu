@@ -17,8 +17,12 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kGroupLanes = 16;     // lanes of a 128-column group
-constexpr int kRowsPerWarp = 4;     // activation rows a warp has in flight
-constexpr int kRowsPerCta = kRowsPerWarp * kThreads / 32;
+// Activation rows a warp has in flight: the 16 lanes of a half warp do the two
+// divisions of eight 16-bit rows; four fp32 rows are as many registers.
+template <typename T>
+constexpr int kRowsPerWarp = sizeof(T) == 4 ? 4 : 8;
+template <typename T>
+constexpr int kRowsPerCta = kRowsPerWarp<T> * kThreads / 32;
 
 // A lane's eight elements of a group as they lie in memory.
 template <typename T>
@@ -41,15 +45,19 @@ S3T_DEV int lane_col(int lane16, int i) {
     return VEC ? lane16 * 8 + i : lane16 + 16 * i;
 }
 
+template <typename T>
+S3T_DEV void load_raw(const T* p, Raw<T>& v) {
+#pragma unroll
+    for (int i = 0; i < int(sizeof(T)) / 2; ++i) {
+        const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+        v.w[4 * i] = u.x; v.w[4 * i + 1] = u.y; v.w[4 * i + 2] = u.z; v.w[4 * i + 3] = u.w;
+    }
+}
+
 template <typename T, bool VEC>
 S3T_DEV void load_group(const T* row, int64_t c0, int64_t cols, int lane16, Raw<T>& v) {
     if (VEC && c0 + lane16 * 8 + 8 <= cols) {
-        const uint4* p = reinterpret_cast<const uint4*>(row + c0 + lane16 * 8);
-#pragma unroll
-        for (int i = 0; i < int(sizeof(T)) / 2; ++i) {
-            const uint4 u = p[i];
-            v.w[4 * i] = u.x; v.w[4 * i + 1] = u.y; v.w[4 * i + 2] = u.z; v.w[4 * i + 3] = u.w;
-        }
+        load_raw(row + c0 + lane16 * 8, v);
         return;
     }
     T e[8];
@@ -67,20 +75,25 @@ S3T_DEV void no_group(Raw<T>& v) {
     for (int i = 0; i < int(2 * sizeof(T)); ++i) v.w[i] = 0;
 }
 
-template <typename T, bool VEC>
-S3T_DEV void store_group(uint8_t* row, int64_t c0, int64_t cols, int lane16, const Raw<T>& v, float inv) {
+template <typename T>
+S3T_DEV uint2 codes(const Raw<T>& v, float inv) {
     float2 f[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = __fmul2_rn(elements(v, i), make_float2(inv, inv));
-    const uint32_t lo = pack_e4m3x4(f[0].x, f[0].y, f[1].x, f[1].y), hi = pack_e4m3x4(f[2].x, f[2].y, f[3].x, f[3].y);
+    return make_uint2(pack_e4m3x4(f[0].x, f[0].y, f[1].x, f[1].y), pack_e4m3x4(f[2].x, f[2].y, f[3].x, f[3].y));
+}
+
+template <typename T, bool VEC>
+S3T_DEV void store_group(uint8_t* row, int64_t c0, int64_t cols, int lane16, const Raw<T>& v, float inv) {
+    const uint2 c = codes(v, inv);
     if (VEC && c0 + lane16 * 8 + 8 <= cols) {
-        *reinterpret_cast<uint2*>(row + c0 + lane16 * 8) = make_uint2(lo, hi);
+        *reinterpret_cast<uint2*>(row + c0 + lane16 * 8) = c;
         return;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const int64_t c = c0 + lane_col<VEC>(lane16, i);
-        if (c < cols) row[c] = uint8_t((i < 4 ? lo : hi) >> (8 * (i & 3)));
+        const int64_t at = c0 + lane_col<VEC>(lane16, i);
+        if (at < cols) row[at] = uint8_t((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
     }
 }
 
@@ -107,56 +120,75 @@ S3T_DEV uint32_t float_bits(uint32_t peak) {
     else return __float_as_uint(unpack2(peak, T()).x);
 }
 
-// A warp takes two groups (256 columns) of four consecutive rows.  The maxima
-// of two 16-bit rows share a word in the reduction, and each lane does one of
-// the eight divisions (a / 448 and 448 / a of four rows) of its half warp.
+// A warp takes two groups (256 columns) of kRowsPerWarp consecutive rows.  The
+// maxima of two 16-bit rows share a word in the reduction, and each lane does
+// one of the divisions (a / 448 and 448 / a of each row) of its half warp.
+// INSIDE: all of the warp's rows and columns are there (nearly every warp of a
+// large matrix), so no access is guarded: at 6.5 TB/s the kernel issues on four
+// of five clocks, and its instructions are what the 1 kW cap slows down.
+template <typename T, bool VEC, bool INSIDE>
+S3T_DEV void quantize_rows(const QuantizeArgs& a, int64_t r0, int64_t g, int lane16) {
+    constexpr int ROWS = kRowsPerWarp<T>;
+    const int64_t c0 = g * kScaleBlock;
+    Raw<T> v[ROWS];
+    {
+        const T* x = static_cast<const T*>(a.x) + r0 * a.x_stride;
+        if constexpr (INSIDE) x += c0 + lane16 * 8;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            // Rows and columns past the end read nothing and count as zeros.
+            if constexpr (INSIDE) load_raw(x, v[r]);
+            else if (r0 + r < a.rows) load_group<T, VEC>(x, c0, a.cols, lane16, v[r]);
+            else no_group(v[r]);
+            x += a.x_stride;
+        }
+    }
+    // Bits of row k's largest magnitude: a word each, or two rows a word.
+    constexpr int WORDS = sizeof(T) == 4 ? ROWS : ROWS / 2;
+    uint32_t peak[WORDS];
+#pragma unroll
+    for (int k = 0; k < WORDS; ++k) {
+        if constexpr (sizeof(T) == 4) peak[k] = peak_bits(v[k]);
+        else peak[k] = peak_bits(v[2 * k]) | (peak_bits(v[2 * k + 1]) << 16);
+    }
+#pragma unroll
+    for (int o = kGroupLanes / 2; o; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < WORDS; ++k) {
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, peak[k], o);
+            peak[k] = sizeof(T) == 4 ? max(peak[k], other) : __vmaxu2(peak[k], other);
+        }
+    const int row = lane16 & (ROWS - 1);
+    uint32_t mine = peak[0];
+#pragma unroll
+    for (int k = 1; k < WORDS; ++k)
+        if (row / (ROWS / WORDS) == k) mine = peak[k];
+    if constexpr (sizeof(T) != 4) mine = row & 1 ? mine >> 16 : mine & 0xffffu;
+    const float top = __uint_as_float(max(float_bits<T>(mine), kAmaxFloorBits));
+    const bool inverse = lane16 & ROWS;
+    const float quotient = __fdiv_rn(inverse ? kE4M3Max : top, inverse ? top : kE4M3Max);
+    uint8_t* q = a.q + r0 * a.q_stride;
+    if constexpr (INSIDE) q += c0 + lane16 * 8;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        const float inv = __shfl_sync(0xffffffffu, quotient, ROWS + r, kGroupLanes);
+        if constexpr (INSIDE) *reinterpret_cast<uint2*>(q) = codes(v[r], inv);
+        else if (r0 + r < a.rows && c0 < a.cols) store_group<T, VEC>(q, c0, a.cols, lane16, v[r], inv);
+        q += a.q_stride;
+    }
+    if (lane16 < ROWS && (INSIDE || (r0 + row < a.rows && c0 < a.cols))) a.scale[g * a.scale_stride + r0 + row] = quotient;
+}
+
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 8) quantize_rows_kernel(const QuantizeArgs a, uint32_t col_blocks) {
+__global__ void __launch_bounds__(kThreads, 4) quantize_rows_kernel(const QuantizeArgs a, uint32_t col_blocks) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rb = blockIdx.x / col_blocks, cb = blockIdx.x - rb * col_blocks;
-    const int64_t r0 = int64_t(rb) * kRowsPerCta + warp * kRowsPerWarp;
-    const int lane16 = lane % kGroupLanes;
+    const int64_t r0 = int64_t(rb) * kRowsPerCta<T> + warp * kRowsPerWarp<T>;
     const int64_t g = int64_t(cb) * 2 + lane / kGroupLanes;
-    const int64_t c0 = g * kScaleBlock;
-    const T* x = static_cast<const T*>(a.x) + r0 * a.x_stride;
-    Raw<T> v[kRowsPerWarp];
-    // Rows and columns past the end read nothing and count as zeros.
-#pragma unroll
-    for (int r = 0; r < kRowsPerWarp; ++r) {
-        if (r0 + r < a.rows) load_group<T, VEC>(x + r * a.x_stride, c0, a.cols, lane16, v[r]);
-        else no_group(v[r]);
-    }
-    uint32_t peak[kRowsPerWarp];
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int r = 0; r < kRowsPerWarp; ++r) peak[r] = peak_bits(v[r]);
-#pragma unroll
-        for (int o = kGroupLanes / 2; o; o >>= 1)
-#pragma unroll
-            for (int r = 0; r < kRowsPerWarp; ++r) peak[r] = max(peak[r], __shfl_xor_sync(0xffffffffu, peak[r], o));
-    } else {
-        uint32_t two[kRowsPerWarp / 2];
-#pragma unroll
-        for (int r = 0; r < kRowsPerWarp / 2; ++r) two[r] = peak_bits(v[2 * r]) | (peak_bits(v[2 * r + 1]) << 16);
-#pragma unroll
-        for (int o = kGroupLanes / 2; o; o >>= 1)
-#pragma unroll
-            for (int r = 0; r < kRowsPerWarp / 2; ++r) two[r] = __vmaxu2(two[r], __shfl_xor_sync(0xffffffffu, two[r], o));
-#pragma unroll
-        for (int r = 0; r < kRowsPerWarp; ++r) peak[r] = r & 1 ? two[r / 2] >> 16 : two[r / 2] & 0xffffu;
-    }
-    static_assert(kRowsPerWarp == 4, "lane pattern of the divisions");
-    const int row = lane16 & 3;
-    const uint32_t mine = row & 2 ? (row & 1 ? peak[3] : peak[2]) : (row & 1 ? peak[1] : peak[0]);
-    const float top = __uint_as_float(max(float_bits<T>(mine), kAmaxFloorBits));
-    const bool inverse = lane16 & 4;
-    const float quotient = __fdiv_rn(inverse ? kE4M3Max : top, inverse ? top : kE4M3Max);
-#pragma unroll
-    for (int r = 0; r < kRowsPerWarp; ++r) {
-        const float inv = __shfl_sync(0xffffffffu, quotient, 4 + r, kGroupLanes);
-        if (r0 + r < a.rows && c0 < a.cols) store_group<T, VEC>(a.q + (r0 + r) * a.q_stride, c0, a.cols, lane16, v[r], inv);
-    }
-    if (lane16 < 4 && r0 + row < a.rows && c0 < a.cols) a.scale[g * a.scale_stride + r0 + row] = quotient;
+    if (VEC && r0 + kRowsPerWarp<T> <= a.rows && int64_t(cb + 1) * 2 * kScaleBlock <= a.cols)
+        quantize_rows<T, VEC, VEC>(a, r0, g, lane % kGroupLanes);
+    else
+        quantize_rows<T, VEC, false>(a, r0, g, lane % kGroupLanes);
 }
 
 // A CTA takes one 128 x 128 block: 16 rows at a time, eight times, all in registers.
@@ -197,7 +229,7 @@ template <typename T, bool VEC>
 cudaError_t launch(const QuantizeArgs& a, cudaStream_t stream) {
     const bool blocks = a.block_rows != 1;
     const int64_t cb = (a.cols + (blocks ? kScaleBlock : 2 * kScaleBlock) - 1) / (blocks ? kScaleBlock : 2 * kScaleBlock);
-    const int64_t rb = (a.rows + (blocks ? kScaleBlock : kRowsPerCta) - 1) / (blocks ? kScaleBlock : kRowsPerCta);
+    const int64_t rb = (a.rows + (blocks ? kScaleBlock : kRowsPerCta<T>) - 1) / (blocks ? kScaleBlock : kRowsPerCta<T>);
     if (rb > 0x7fffffff / cb) return cudaErrorInvalidValue;
     if (blocks)
         quantize_blocks_kernel<T, VEC><<<uint32_t(rb * cb), kThreads, 0, stream>>>(a, uint32_t(cb));
