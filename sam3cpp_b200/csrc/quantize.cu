@@ -54,6 +54,32 @@ S3T_DEV void load_raw(const T* p, Raw<T>& v) {
     }
 }
 
+// Eight consecutive elements at any address, from the whole 16-byte units that
+// hold them (a unit with one of the row's bytes lies in the row's allocation).
+template <typename T>
+S3T_DEV void load_shifted(const T* p, Raw<T>& v) {
+    constexpr int WORDS = 2 * int(sizeof(T));
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    const uint32_t shift = uint32_t(at) & 15;
+    const uint4* units = reinterpret_cast<const uint4*>(at - shift);
+    uint32_t c[WORDS + 4];
+#pragma unroll
+    for (int i = 0; i <= WORDS / 4; ++i) {
+        const uint4 u = i < WORDS / 4 || shift ? units[i] : make_uint4(0, 0, 0, 0);
+        c[4 * i] = u.x; c[4 * i + 1] = u.y; c[4 * i + 2] = u.z; c[4 * i + 3] = u.w;
+    }
+    if (shift & 8) {
+#pragma unroll
+        for (int i = 0; i + 2 < WORDS + 4; ++i) c[i] = c[i + 2];
+    }
+    if (shift & 4) {
+#pragma unroll
+        for (int i = 0; i + 1 < WORDS + 4; ++i) c[i] = c[i + 1];
+    }
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) v.w[i] = sizeof(T) < 4 && (shift & 2) ? __funnelshift_r(c[i], c[i + 1], 16) : c[i];
+}
+
 template <typename T, bool VEC>
 S3T_DEV void load_group(const T* row, int64_t c0, int64_t cols, int lane16, Raw<T>& v) {
     if (VEC && c0 + lane16 * 8 + 8 <= cols) {
@@ -137,7 +163,8 @@ S3T_DEV void quantize_rows(const QuantizeArgs& a, int64_t r0, int64_t g, int lan
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             // Rows and columns past the end read nothing and count as zeros.
-            if constexpr (INSIDE) load_raw(x, v[r]);
+            if constexpr (INSIDE && VEC) load_raw(x, v[r]);
+            else if constexpr (INSIDE) load_shifted(x, v[r]);
             else if (r0 + r < a.rows) load_group<T, VEC>(x, c0, a.cols, lane16, v[r]);
             else no_group(v[r]);
             x += a.x_stride;
@@ -185,8 +212,8 @@ __global__ void __launch_bounds__(kThreads, 4) quantize_rows_kernel(const Quanti
     const uint32_t rb = blockIdx.x / col_blocks, cb = blockIdx.x - rb * col_blocks;
     const int64_t r0 = int64_t(rb) * kRowsPerCta<T> + warp * kRowsPerWarp<T>;
     const int64_t g = int64_t(cb) * 2 + lane / kGroupLanes;
-    if (VEC && r0 + kRowsPerWarp<T> <= a.rows && int64_t(cb + 1) * 2 * kScaleBlock <= a.cols)
-        quantize_rows<T, VEC, VEC>(a, r0, g, lane % kGroupLanes);
+    if (r0 + kRowsPerWarp<T> <= a.rows && int64_t(cb + 1) * 2 * kScaleBlock <= a.cols)
+        quantize_rows<T, VEC, true>(a, r0, g, lane % kGroupLanes);
     else
         quantize_rows<T, VEC, false>(a, r0, g, lane % kGroupLanes);
 }
@@ -201,13 +228,15 @@ __global__ void __launch_bounds__(kThreads) quantize_blocks_kernel(const Quantiz
     const int64_t r0 = int64_t(rb) * kScaleBlock + threadIdx.x / kGroupLanes;
     const int64_t c0 = int64_t(cb) * kScaleBlock;
     const T* x = static_cast<const T*>(a.x);
+    const bool inside = c0 + kScaleBlock <= a.cols;   // all columns are there
     Raw<T> v[kPasses];
     uint32_t m = 0;
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
         const int64_t r = r0 + p * (kThreads / kGroupLanes);
-        if (r < a.rows) load_group<T, VEC>(x + r * a.x_stride, c0, a.cols, lane16, v[p]);
-        else no_group(v[p]);
+        if (r >= a.rows) no_group(v[p]);
+        else if (!VEC && inside) load_shifted(x + r * a.x_stride + c0 + lane16 * 8, v[p]);
+        else load_group<T, VEC>(x + r * a.x_stride, c0, a.cols, lane16, v[p]);
     }
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) m = max(m, peak_bits(v[p]));
@@ -221,7 +250,9 @@ __global__ void __launch_bounds__(kThreads) quantize_blocks_kernel(const Quantiz
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
         const int64_t r = r0 + p * (kThreads / kGroupLanes);
-        if (r < a.rows) store_group<T, VEC>(a.q + r * a.q_stride, c0, a.cols, lane16, v[p], s.inv);
+        if (r >= a.rows) continue;
+        if (!VEC && inside) store_group<T, true>(a.q + r * a.q_stride, c0, a.cols, lane16, v[p], s.inv);
+        else store_group<T, VEC>(a.q + r * a.q_stride, c0, a.cols, lane16, v[p], s.inv);
     }
 }
 
