@@ -264,8 +264,9 @@ int s3t_layernorm(int device, const float *x, int rows, const float *gamma, cons
  * workspace, so calls may overlap on several streams and be captured.  The
  * first call of any entry point on a device prepares that device (allocates):
  * make it before a capture.  The caller's current device is left as it was.
- * Strides count elements.  Outputs overlap no input, except where in place is
- * allowed below.  A call with no rows or tokens (or no columns) writes nothing
+ * Strides count elements.  Inputs are read in whole 16-byte units that hold one
+ * of their bytes.  Outputs overlap no input, except where in place is allowed
+ * below.  A call with no rows or tokens (or no columns) writes nothing
  * and succeeds. */
 
 /* Rows of a matrix in device memory.  scale and scale_stride belong to e4m3

@@ -31,6 +31,8 @@
 #include "fp8.cuh"
 #include "kernels.h"
 
+#include <type_traits>
+
 namespace s3t {
 
 namespace {
@@ -350,11 +352,24 @@ __global__ void __launch_bounds__(32 * kMaxWarps) norm_rows_kernel(const NormRes
 template <typename T, typename R>
 struct StreamRow {
     static constexpr uint32_t COLS = kStreamCpw * kChunk;
-    static constexpr uint32_t X = COLS * sizeof(R), Y = COLS * sizeof(T);
+    static constexpr uint32_t X = COLS * sizeof(R) + 16, Y = COLS * sizeof(T) + 16;   // and what lies around them
     static constexpr uint32_t BYTES = X + 2 * Y;
 };
 
-template <typename T, typename R>
+// The 16-byte units that hold `bytes` bytes from p on; returns their size.
+S3T_DEV uint32_t bulk_load_around(uint8_t* to, const void* p, uint32_t bytes, uint64_t* bar) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p), first = at & ~uintptr_t(15);
+    const uint32_t size = (uint32_t(at - first) + bytes + 15) & ~15u;
+    bulk_load(to, reinterpret_cast<const void*>(first), size, bar);
+    return size;
+}
+S3T_DEV uint32_t units_around(const void* p, uint32_t bytes) {
+    return ((uint32_t(reinterpret_cast<uintptr_t>(p)) & 15) + bytes + 15) & ~15u;
+}
+
+// VEC: rows and columns in whole 16-byte units; else the units around a row
+// come, and a lane picks its elements from where the row begins in them.
+template <typename T, typename R, bool VEC>
 __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const NormResidualArgs a) {
     constexpr int CPW = kStreamCpw;
     using Row = StreamRow<T, R>;
@@ -377,7 +392,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
                 vec[k * padded + c] = c < dim ? (from[k] ? from[k][c] : otherwise) * times : 0.f;
         }
     }
-    // Columns past dim are never copied: they stay zeros.
+    // VEC: columns past dim are never copied, they stay zeros.
     uint8_t* mine = reinterpret_cast<uint8_t*>(vec + kVectors * padded) + (team * warps + warp) * kSlots * Row::BYTES;
     for (uint32_t i = lane; i < kSlots * Row::BYTES / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
     uint64_t* bar = arrived[team * warps + warp];
@@ -399,13 +414,14 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
     auto fetch = [&](int slot) {       // one lane
         if (ahead >= rows) return;
         uint8_t* to = mine + slot * Row::BYTES;
-        mbar_arrive_expect_tx(bar + slot, uint32_t(cols) * (sizeof(R) + (a.y ? sizeof(T) : 0) + (a.gate ? sizeof(T) : 0)));
-        if (a.y) bulk_load(to + Row::X, yp, cols * sizeof(T), bar + slot);
-        bulk_load(to, xp, cols * sizeof(R), bar + slot);
-        if (a.gate)
-            bulk_load(to + Row::X + Row::Y,
-                      static_cast<const T*>(a.gate) + int64_t(ahead / uint32_t(a.gate_rows)) * a.gate_stride + c0,
-                      cols * sizeof(T), bar + slot);
+        const uint32_t xb = uint32_t(cols) * sizeof(R), tb = uint32_t(cols) * sizeof(T);
+        const T* gp = static_cast<const T*>(a.gate);
+        if (a.gate) gp += int64_t(ahead / uint32_t(a.gate_rows)) * a.gate_stride + c0;
+        mbar_arrive_expect_tx(bar + slot, units_around(xp, xb) + (a.y ? units_around(yp, tb) : 0) +
+                                              (a.gate ? units_around(gp, tb) : 0));
+        if (a.y) bulk_load_around(to + Row::X, yp, tb, bar + slot);
+        bulk_load_around(to, xp, xb, bar + slot);
+        if (a.gate) bulk_load_around(to + Row::X + Row::Y, gp, tb, bar + slot);
         xp += x_step;
         yp += y_step;
         ahead = rows - ahead > stride ? ahead + stride : rows;
@@ -421,13 +437,19 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
         lost = lost || !mbar_wait(bar + slot, (it / kSlots) & 1, a.status, kErrTimeoutProducer, nullptr);
         const uint8_t* from = mine + slot * Row::BYTES;
         float2 x[CPW][4], h[CPW][4];
-        auto vector = [&](int k, int j, float2(&v)[4]) { load_chunk<true>(vec + k * padded + c0 + j * kChunk, 0, kChunk, lane, v); };
+        auto vector = [&](int k, int j, float2(&v)[4]) { load_chunk<VEC>(vec + k * padded + c0 + j * kChunk, 0, kChunk, lane, v); };
+        // Chunk j of a row whose units lie at p and which begins where `at` says.
+        auto chunk = [&](const uint8_t* p, auto* at, int j, float2(&v)[4]) {
+            using E = typename std::remove_const<typename std::remove_pointer<decltype(at)>::type>::type;
+            if constexpr (VEC) load_chunk<true>(reinterpret_cast<const E*>(p) + j * kChunk, 0, kChunk, lane, v);
+            else load_chunk<false>(reinterpret_cast<const E*>(p + (reinterpret_cast<uintptr_t>(at) & 15)), j * kChunk, cols, lane, v);
+        };
         if (a.y) {
 #pragma unroll
             for (int j = 0; j < CPW; ++j)
-                load_chunk<true>(reinterpret_cast<const T*>(from + Row::X) + j * kChunk, 0, kChunk, lane, h[j]);
+                chunk(from + Row::X, static_cast<const T*>(a.y) + int64_t(row) * a.y_stride + c0, j, h[j]);
             if (a.post) {
-                const RowStats st = row_stats<CPW, true>(h, a.layer, dim, a.eps, sp, exchange[team][it & 1][0]);
+                const RowStats st = row_stats<CPW, VEC>(h, a.layer, dim, a.eps, sp, exchange[team][it & 1][0]);
 #pragma unroll
                 for (int j = 0; j < CPW; ++j) {
                     float2 w[4], b[4];
@@ -440,14 +462,15 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
 #pragma unroll
                 for (int j = 0; j < CPW; ++j) {
                     float2 g[4];
-                    load_chunk<true>(reinterpret_cast<const T*>(from + Row::X + Row::Y) + j * kChunk, 0, kChunk, lane, g);
+                    chunk(from + Row::X + Row::Y,
+                          static_cast<const T*>(a.gate) + int64_t(row / uint32_t(a.gate_rows)) * a.gate_stride + c0, j, g);
                     apply_gate(h[j], g, a.gate_act);
                 }
             }
         }
 #pragma unroll
         for (int j = 0; j < CPW; ++j) {
-            load_chunk<true>(reinterpret_cast<const R*>(from) + j * kChunk, 0, kChunk, lane, x[j]);
+            chunk(from, static_cast<const R*>(a.x) + int64_t(row) * a.x_stride + c0, j, x[j]);
             if (a.y) {
                 float2 s[4];
                 vector(2, j, s);
@@ -463,12 +486,12 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
         if (a.x_out) {
 #pragma unroll
             for (int j = 0; j < CPW; ++j) {
-                if (whole) store_chunk<true>(xo + j * kChunk, 0, kChunk, lane, x[j]);
-                else store_chunk<true>(xo, j * kChunk, cols, lane, x[j]);
+                if (whole) store_chunk<VEC>(xo + j * kChunk, 0, kChunk, lane, x[j]);
+                else store_chunk<VEC>(xo, j * kChunk, cols, lane, x[j]);
             }
         }
         if (a.u) {
-            const RowStats st = row_stats<CPW, true>(x, a.layer, dim, a.eps, sp, exchange[team][it & 1][1]);
+            const RowStats st = row_stats<CPW, VEC>(x, a.layer, dim, a.eps, sp, exchange[team][it & 1][1]);
 #pragma unroll
             for (int j = 0; j < CPW; ++j) {
                 float2 w[4], b[4];
@@ -476,9 +499,9 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
                 vector(4, j, b);
                 normalize(x[j], st, w, b);
                 if (!a.u_eight)
-                    store_chunk<true>(static_cast<T*>(a.u) + int64_t(row) * a.u_stride, c0 + j * kChunk, dim, lane, x[j]);
+                    store_chunk<VEC>(static_cast<T*>(a.u) + int64_t(row) * a.u_stride, c0 + j * kChunk, dim, lane, x[j]);
             }
-            if (a.u_eight) store_eight<CPW, true>(a, row, c0, lane, x);
+            if (a.u_eight) store_eight<CPW, VEC>(a, row, c0, lane, x);
         }
         xo += xo_step;
         row = rows - row > stride ? row + stride : rows;
@@ -502,9 +525,11 @@ cudaError_t launch_types(const NormResidualArgs& a, int num_sms, cudaStream_t st
     int teams = vector_bytes < kStreamBytes ? (kStreamBytes - vector_bytes) / (warps * kSlots * int(Row::BYTES)) : 0;
     if (teams > kStreamWarps / warps) teams = kStreamWarps / warps;
     // Two rows a team and more: the rows ahead pay for the set-up.
-    if (a.vec && teams > 0 && a.rows >= int64_t(2) * num_sms * teams) {
-        norm_stream_kernel<T, R><<<num_sms, dim3(32 * warps, teams),
-                                   uint32_t(vector_bytes) + uint32_t(teams * warps) * kSlots * Row::BYTES, stream>>>(a);
+    if (a.dim > kChunk && teams > 0 && a.rows >= int64_t(2) * num_sms * teams) {
+        const dim3 block(32 * warps, teams);
+        const uint32_t smem = uint32_t(vector_bytes) + uint32_t(teams * warps) * kSlots * Row::BYTES;
+        if (a.vec) norm_stream_kernel<T, R, true><<<num_sms, block, smem, stream>>>(a);
+        else norm_stream_kernel<T, R, false><<<num_sms, block, smem, stream>>>(a);
         return cudaGetLastError();
     }
     if (a.dim <= kMaxWarps * kChunk) return a.vec ? launch_few<T, R, 1, true>(a, stream) : launch_few<T, R, 1, false>(a, stream);
@@ -513,7 +538,10 @@ cudaError_t launch_types(const NormResidualArgs& a, int num_sms, cudaStream_t st
 
 template <typename T, typename R>
 cudaError_t prepare_types() {
-    return cudaFuncSetAttribute(norm_stream_kernel<T, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamBytes);
+    const cudaError_t e =
+        cudaFuncSetAttribute(norm_stream_kernel<T, R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamBytes);
+    if (e != cudaSuccess) return e;
+    return cudaFuncSetAttribute(norm_stream_kernel<T, R, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamBytes);
 }
 
 }  // namespace

@@ -387,6 +387,16 @@ def test_norm_many_rows(torch, rows, dim):
     run_norm(torch, 9, rows, dim, "bf16", "bf16", gate="none")
 
 
+@pytest.mark.parametrize("kind, resid", TYPE_PAIRS)
+@pytest.mark.parametrize("rows, dim, pad", [(5000, 1024, 0), (4800, 264, 0), (4741, 1001, 0), (4740, 515, 3), (2400, 2050, 1),
+                                            (1300, 4735, 0), (4739, 257, 16)])
+def test_norm_streams_of_rows(torch, kind, resid, rows, dim, pad):
+    """Enough rows for the persistent kernel (two a team), aligned and at any address."""
+    run_norm(torch, 10, rows, dim, kind, resid, layer=True, gate="plain", gate_rows=7, eight=True, pad=pad)
+    run_norm(torch, 11, rows, dim, kind, resid, gate="tanh", gate_rows=1000, pad=pad, in_place=True, resid_scale=0.5)
+    run_norm(torch, 12, rows, dim, kind, resid, branch=False, layer=True, weights=False, pad=pad, write_x=False)
+
+
 def test_norm_parts_that_are_left_out(torch):
     for dim in (256, 515):
         run_norm(torch, 1, 9, dim, "f16", "f32", branch=False)                                  # a pre-norm alone
@@ -405,7 +415,7 @@ def test_norm_far_from_zero(torch):
 
 
 def test_norm_nonfinite_rows_stay_apart(torch):
-    for rows, dim in ((5, 1024), (2100, 512), (5, 301)):
+    for rows, dim in ((5, 1024), (2100, 512), (5, 301), (5000, 512), (5000, 1003)):
         x = torch.randn(rows, dim, device="cuda")
         x[1, 3], x[2, 4] = float("nan"), float("inf")
         u = torch.empty(rows, dim, device="cuda")
