@@ -13,8 +13,8 @@
 // access of a warp is contiguous and a scale group's maximum is one warp
 // reduction); warp w of a row's team holds CPW consecutive chunks.
 //
-// Many rows (STREAM): persistent CTAs, four chunks a warp, so that a reduction
-// or a barrier is paid once for 32 columns a lane; the vectors wait in shared
+// Many rows (STREAM): persistent CTAs, up to four chunks a warp, so that a
+// reduction or a barrier is paid once for 32 columns a lane; the vectors wait in shared
 // memory and the next row comes there by bulk copies while the second half of
 // a row is computed.  82944 x 1024, LayerNorm twice, gate, e4m3 out: 158 us,
 // 5.9 TB/s with 16 warps an SM and one row ahead (12 warps and two rows: 174
@@ -40,7 +40,6 @@ namespace {
 constexpr int kChunk = 2 * kScaleBlock;
 constexpr int kMaxWarps = 16;          // of a team: 16 x 4 chunks hold kNormMaxDim columns
 constexpr int kSlots = 1;              // rows ahead of a warp (STREAM)
-constexpr int kStreamCpw = 4;
 constexpr int kStreamWarps = 16;
 constexpr int kStreamBytes = 200 * 1024;
 constexpr int kVectors = 5;            // post weight and bias, branch factor, pre weight and bias
@@ -349,9 +348,9 @@ __global__ void __launch_bounds__(32 * kMaxWarps) norm_rows_kernel(const NormRes
 // Shared memory of a streaming CTA: the vectors, each a row of floats padded
 // to its team's columns; then per warp kSlots rows of its columns of x, y and
 // gate; then the barriers.
-template <typename T, typename R>
+template <typename T, typename R, int CPW>
 struct StreamRow {
-    static constexpr uint32_t COLS = kStreamCpw * kChunk;
+    static constexpr uint32_t COLS = CPW * kChunk;
     static constexpr uint32_t X = COLS * sizeof(R) + 16, Y = COLS * sizeof(T) + 16;   // and what lies around them
     static constexpr uint32_t BYTES = X + 2 * Y;
 };
@@ -369,10 +368,9 @@ S3T_DEV uint32_t units_around(const void* p, uint32_t bytes) {
 
 // VEC: rows and columns in whole 16-byte units; else the units around a row
 // come, and a lane picks its elements from where the row begins in them.
-template <typename T, typename R, bool VEC>
+template <typename T, typename R, int CPW, bool VEC>
 __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const NormResidualArgs a) {
-    constexpr int CPW = kStreamCpw;
-    using Row = StreamRow<T, R>;
+    using Row = StreamRow<T, R, CPW>;
     // Two parities: a slot is written again two barriers after its last read.
     __shared__ float2 exchange[kStreamWarps][2][2][kStreamWarps];
     __shared__ uint64_t arrived[kStreamWarps][kSlots];
@@ -517,31 +515,47 @@ cudaError_t launch_few(const NormResidualArgs& a, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
-template <typename T, typename R>
-cudaError_t launch_types(const NormResidualArgs& a, int num_sms, cudaStream_t stream) {
-    using Row = StreamRow<T, R>;
+// The streaming kernel for rows of CPW chunks a warp; false: not for this call.
+template <typename T, typename R, int CPW>
+bool launch_stream(const NormResidualArgs& a, int num_sms, cudaStream_t stream) {
+    using Row = StreamRow<T, R, CPW>;
     const int warps = (a.dim + int(Row::COLS) - 1) / int(Row::COLS);
     const int vector_bytes = kVectors * warps * int(Row::COLS) * 4;
     int teams = vector_bytes < kStreamBytes ? (kStreamBytes - vector_bytes) / (warps * kSlots * int(Row::BYTES)) : 0;
     if (teams > kStreamWarps / warps) teams = kStreamWarps / warps;
     // Two rows a team and more: the rows ahead pay for the set-up.
-    if (a.dim > kChunk && teams > 0 && a.rows >= int64_t(2) * num_sms * teams) {
-        const dim3 block(32 * warps, teams);
-        const uint32_t smem = uint32_t(vector_bytes) + uint32_t(teams * warps) * kSlots * Row::BYTES;
-        if (a.vec) norm_stream_kernel<T, R, true><<<num_sms, block, smem, stream>>>(a);
-        else norm_stream_kernel<T, R, false><<<num_sms, block, smem, stream>>>(a);
-        return cudaGetLastError();
-    }
+    if (teams == 0 || a.rows < int64_t(2) * num_sms * teams) return false;
+    const dim3 block(32 * warps, teams);
+    const uint32_t smem = uint32_t(vector_bytes) + uint32_t(teams * warps) * kSlots * Row::BYTES;
+    if (a.vec) norm_stream_kernel<T, R, CPW, true><<<num_sms, block, smem, stream>>>(a);
+    else norm_stream_kernel<T, R, CPW, false><<<num_sms, block, smem, stream>>>(a);
+    return true;
+}
+
+template <typename T, typename R>
+cudaError_t launch_types(const NormResidualArgs& a, int num_sms, cudaStream_t stream) {
+    const bool streamed = a.dim <= kChunk       ? launch_stream<T, R, 1>(a, num_sms, stream)
+                          : a.dim <= 2 * kChunk ? launch_stream<T, R, 2>(a, num_sms, stream)
+                                                : launch_stream<T, R, 4>(a, num_sms, stream);
+    if (streamed) return cudaGetLastError();
     if (a.dim <= kMaxWarps * kChunk) return a.vec ? launch_few<T, R, 1, true>(a, stream) : launch_few<T, R, 1, false>(a, stream);
     return a.vec ? launch_few<T, R, 4, true>(a, stream) : launch_few<T, R, 4, false>(a, stream);
 }
 
+template <typename T, typename R, int CPW>
+cudaError_t prepare_stream() {
+    const cudaError_t e =
+        cudaFuncSetAttribute(norm_stream_kernel<T, R, CPW, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamBytes);
+    if (e != cudaSuccess) return e;
+    return cudaFuncSetAttribute(norm_stream_kernel<T, R, CPW, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamBytes);
+}
+
 template <typename T, typename R>
 cudaError_t prepare_types() {
-    const cudaError_t e =
-        cudaFuncSetAttribute(norm_stream_kernel<T, R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamBytes);
-    if (e != cudaSuccess) return e;
-    return cudaFuncSetAttribute(norm_stream_kernel<T, R, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamBytes);
+    cudaError_t e;
+    if ((e = prepare_stream<T, R, 1>()) != cudaSuccess) return e;
+    if ((e = prepare_stream<T, R, 2>()) != cudaSuccess) return e;
+    return prepare_stream<T, R, 4>();
 }
 
 }  // namespace

@@ -389,7 +389,8 @@ def test_norm_many_rows(torch, rows, dim):
 
 @pytest.mark.parametrize("kind, resid", TYPE_PAIRS)
 @pytest.mark.parametrize("rows, dim, pad", [(5000, 1024, 0), (4800, 264, 0), (4741, 1001, 0), (4740, 515, 3), (2400, 2050, 1),
-                                            (1300, 4735, 0), (4739, 257, 16)])
+                                            (1300, 4735, 0), (4739, 257, 16), (4745, 130, 0), (4737, 7, 1), (4800, 256, 0),
+                                            (4736, 500, 4)])
 def test_norm_streams_of_rows(torch, kind, resid, rows, dim, pad):
     """Enough rows for the persistent kernel (two a team), aligned and at any address."""
     run_norm(torch, 10, rows, dim, kind, resid, layer=True, gate="plain", gate_rows=7, eight=True, pad=pad)
