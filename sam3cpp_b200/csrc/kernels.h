@@ -285,7 +285,7 @@ struct RotaryArgs {
     int kind;                 // ElementKind: kF32, kF16 or kBF16
     int head_dim;
     int interleaved, inverse;
-    int vec;                  // 16-byte aligned heads, whole vectors on both sides of `rot`
+    int run;                  // elements that every access may take: 16 bytes of them, 2 or 1
     RotaryPart part[2];       // part[1].heads may be 0
 };
 constexpr int kRotaryMaxDim = 1024;

@@ -263,9 +263,10 @@ int s3t_rotary(int device, const double* freq, int rot_dim, float magnitude, con
         if (!freq || !aligned(freq, 8)) return refuse(op, "freq must be an aligned device pointer");
         if (!positions || !aligned(positions, 8)) return refuse(op, "positions must be an aligned device pointer");
         if (!q) return refuse(op, "q must not be null");
-        const int eb = element_bytes(kind), v = 16 / eb;
+        const int eb = element_bytes(kind);
         RotaryArgs a{};
-        a.vec = (flags & S3T_ROTARY_INTERLEAVED ? rot_dim : rot_dim / 2) % v == 0 && (head_dim - rot_dim) % v == 0;
+        // Everything that a run of elements must divide: columns, strides and addresses.
+        uint64_t marks = uint64_t(flags & S3T_ROTARY_INTERLEAVED ? rot_dim : rot_dim / 2) | uint64_t(head_dim - rot_dim);
         const s3t_rotary_view* const views[2] = {q, k};
         for (int i = 0; i < 2; ++i) {
             const s3t_rotary_view* s = views[i];
@@ -286,9 +287,10 @@ int s3t_rotary(int device, const double* freq, int rot_dim, float magnitude, con
             p.x_head = s->x_head_stride;
             p.out_token = s->out_token_stride;
             p.out_head = s->out_head_stride;
-            a.vec = a.vec && aligned(s->x, 16) && aligned(s->out, 16) && p.x_token % v == 0 && p.x_head % v == 0 &&
-                    p.out_token % v == 0 && p.out_head % v == 0;
+            marks |= (reinterpret_cast<uintptr_t>(s->x) | reinterpret_cast<uintptr_t>(s->out)) / uintptr_t(eb);
+            marks |= uint64_t(p.x_token) | uint64_t(p.x_head) | uint64_t(p.out_token) | uint64_t(p.out_head);
         }
+        a.run = marks % uint64_t(16 / eb) == 0 ? 16 / eb : marks % 2 == 0 ? 2 : 1;
         if (tokens == 0) return 0;
         a.freq = freq;
         a.rot = rot_dim;

@@ -26,20 +26,31 @@ constexpr int kRows = 512;            // heads whose places a CTA holds at a tim
 template <typename T>
 constexpr int kVec = 16 / int(sizeof(T));
 
-// V consecutive elements as they lie in memory: one element, or 16 bytes.
+// V consecutive elements as they lie in memory, moved in one access: one, two,
+// or 16 bytes of them.
+template <int BYTES>
+struct Word;
+template <>
+struct Word<2> { using W = uint16_t; };
+template <>
+struct Word<4> { using W = uint32_t; };
+template <>
+struct Word<8> { using W = uint2; };
+template <>
+struct Word<16> { using W = uint4; };
 template <typename T, int V>
-struct alignas(V == 1 ? alignof(T) : 16) Run {
+struct alignas(V * sizeof(T)) Run {
     T v[V];
 };
 template <typename T, int V>
 S3T_DEV void load_run(const T* p, Run<T, V>& r) {
-    if constexpr (V == 1) r.v[0] = *p;
-    else *reinterpret_cast<uint4*>(r.v) = *reinterpret_cast<const uint4*>(p);
+    using W = typename Word<V * int(sizeof(T))>::W;
+    *reinterpret_cast<W*>(r.v) = *reinterpret_cast<const W*>(p);
 }
 template <typename T, int V>
 S3T_DEV void store_run(T* p, const Run<T, V>& r) {
-    if constexpr (V == 1) *p = r.v[0];
-    else *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(r.v);
+    using W = typename Word<V * int(sizeof(T))>::W;
+    *reinterpret_cast<W*>(p) = *reinterpret_cast<const W*>(r.v);
 }
 template <typename T, int V>
 S3T_DEV void widen(const Run<T, V>& r, float (&v)[V]) {
@@ -216,11 +227,16 @@ cudaError_t launch(const RotaryArgs& a, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
+template <typename T, bool INTERLEAVED>
+cudaError_t launch_run(const RotaryArgs& a, cudaStream_t stream) {
+    if (a.run == kVec<T>) return launch<T, kVec<T>, INTERLEAVED>(a, stream);
+    if (a.run == 2) return launch<T, 2, INTERLEAVED>(a, stream);
+    return launch<T, 1, INTERLEAVED>(a, stream);
+}
+
 template <typename T>
 cudaError_t launch_type(const RotaryArgs& a, cudaStream_t stream) {
-    if (a.interleaved)
-        return a.vec ? launch<T, kVec<T>, true>(a, stream) : launch<T, 1, true>(a, stream);
-    return a.vec ? launch<T, kVec<T>, false>(a, stream) : launch<T, 1, false>(a, stream);
+    return a.interleaved ? launch_run<T, true>(a, stream) : launch_run<T, false>(a, stream);
 }
 
 }  // namespace
