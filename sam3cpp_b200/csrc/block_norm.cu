@@ -16,8 +16,8 @@
 // Many rows (STREAM): persistent CTAs, up to four chunks a warp, so that a
 // reduction or a barrier is paid once for 32 columns a lane; the vectors wait in shared
 // memory and the next row comes there by bulk copies while the second half of
-// a row is computed.  82944 x 1024, LayerNorm twice, gate, e4m3 out: 158 us,
-// 5.9 TB/s with 16 warps an SM and one row ahead (12 warps and two rows: 174
+// a row is computed.  82944 x 1024, LayerNorm twice, gate, e4m3 out: 155 us,
+// 6.0 TB/s with 16 warps an SM and one row ahead (12 warps and two rows: 174
 // us, 20 warps of fewer registers: 168 us); whole rows per warp read straight
 // into registers took 398 us (the loads' latency), one chunk a warp with the
 // next row in registers 269 us (four times the reductions).

@@ -5,8 +5,9 @@
 // Bound by HBM: each element is read once and one byte of it written.  Sixteen
 // lanes hold the 128 columns of a group, eight consecutive elements each, so
 // the group's maximum is four shuffles away and nothing is read twice.  82944 x
-// 4736 fp16: 183 us, 6.5 TB/s (469 us with a division per lane and group and
-// the maxima in fp32: bound by its instructions; 208 us at five CTAs an SM).
+// 4736 fp16: 172 us, 6.9 TB/s (469 us with a division per lane and group and
+// the maxima in fp32: bound by its instructions; 189 us with four rows a warp
+// and every access guarded, 220 us once the 1 kW cap lowers the clocks).
 #include "elements.cuh"
 #include "fp8.cuh"
 #include "kernels.h"
