@@ -470,157 +470,157 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
     const uint32_t tmem_base = *tmem_slot;
 
     if (warp < 4) {
-    setmaxnreg_dec<Cfg::FEW_REGS>();
-    if (warp == 0) {
-        if (lane == 0) {
-            int s = 0;
-            uint32_t ph = 0, armed = 0, armed_parity = 0;
+        setmaxnreg_dec<Cfg::FEW_REGS>();
+        if (warp == 0) {
+            if (lane == 0) {
+                int s = 0;
+                uint32_t ph = 0, armed = 0, armed_parity = 0;
+                bool ok = true;
+                for (int tile = pair; ok && tile < n_tiles; tile += n_pairs) {
+                    const int m0 = (tile / tiles_n) * 2 * kTileM + int(rank) * kTileM;
+                    const int n0 = (tile % tiles_n) * Cfg::BN + int(rank) * kTileM;
+                    for (int g = 0; g < groups; ++g) {
+                        if (!mbar_wait(done + s, ph ^ 1, args.status, kErrTimeoutProducer, abort_flag)) {
+                            ok = false;
+                            break;
+                        }
+                        const uint32_t lfull = mapa_shared(smem_u32(full + s), 0);
+                        if (leader) {
+                            mbar_arrive_expect_tx(full + s, 2 * Cfg::STAGE_BYTES);
+                            armed |= 1u << s;
+                            armed_parity = (armed_parity & ~(1u << s)) | (ph << s);
+                        }
+                        tma_load_2d_pair(sX + s * kHalfBytes, &tmX, lfull, g * kScaleBlock, m0);
+                        tma_load_2d_pair(sW + s * kHalfBytes, &tmW, lfull, g * kScaleBlock, n0);
+                        if (++s == Cfg::STAGES) {
+                            s = 0;
+                            ph ^= 1;
+                        }
+                    }
+                }
+                if (!ok && leader) {
+                    // Gave up: wait (bounded) for the pair's copies counted on these barriers.
+                    for (int i = 0; i < Cfg::STAGES; ++i)
+                        if (armed & (1u << i))
+                            mbar_wait(full + i, (armed_parity >> i) & 1u, args.status, kErrTimeoutDrain, nullptr);
+                }
+            }
+        } else if (warp == 1) {
+            if (leader) {
+                constexpr uint32_t idesc = umma_idesc_e4m3(2 * kTileM, Cfg::BN);
+                const uint64_t dX0 = umma_desc_sw128(smem_u32(sX), 16, 1024);
+                const uint64_t dW0 = umma_desc_sw128(smem_u32(sW), 16, 1024);
+                int s = 0, it = 0;
+                uint32_t ph = 0;
+                bool ok = true, issued = false;
+                for (int tile = pair; ok && tile < n_tiles; tile += n_pairs) {
+                    for (int g = 0; g < groups; ++g, ++it) {
+                        const int acc = it & 1;
+                        const uint32_t aph = (it >> 1) & 1;
+                        if (!mbar_wait(full + s, ph, args.status, kErrTimeoutMma, abort_flag) ||
+                            !mbar_wait(tempty + acc, aph ^ 1, args.status, kErrTimeoutMma, abort_flag)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint64_t dx = dX0 + uint64_t(s) * (kHalfBytes >> 4), dw = dW0 + uint64_t(s) * (kHalfBytes >> 4);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                umma_f8_ss_pair(tmem_base + acc * Cfg::BN, dx + 2 * k, dw + 2 * k, idesc, k != 0);
+                            // One commit per group (a second cost 61 clocks of the tensor
+                            // pipe): the stage is free and its sums are in the accumulator.
+                            umma_commit_pair(done + s, 0x3);
+                        }
+                        __syncwarp();
+                        issued = true;
+                        if (++s == Cfg::STAGES) {
+                            s = 0;
+                            ph ^= 1;
+                        }
+                    }
+                }
+                if (!ok && issued) {
+                    if (elect_one()) umma_commit_pair(drain, 0x1);
+                    __syncwarp();
+                    mbar_wait(drain, 0, args.status, kErrTimeoutDrain, nullptr);
+                }
+            }
+        } else {
+            // Factor warps: xs ws of this CTA's 128 rows and two weight blocks, for
+            // each group, so that a promotion warp reads one word.  The raw scales
+            // come by cp.async, RAW_SLOTS - 1 groups ahead, into words of the
+            // thread's own.  A group's done barrier counts these warps too.
+            const int ft = int(threadIdx.x) - 64;
+            float* mine = raw + ft * 4;
+            int ahead_tile = pair - n_pairs, ahead_left = 0, ahead_slot = 0;
+            const float *x0 = args.xs, *x1 = args.xs, *w0 = args.ws, *w1 = args.ws;
+            bool in_x0 = false, in_x1 = false, in_w0 = false, in_w1 = false;
+            auto fetch = [&]() {
+                if (ahead_left == 0) {
+                    ahead_tile += n_pairs;
+                    const bool tile_ok = ahead_tile < n_tiles;
+                    const int m = tile_ok ? (ahead_tile / tiles_n) * 2 * kTileM + int(rank) * kTileM + ft : 0;
+                    const int n = tile_ok ? (ahead_tile % tiles_n) * Cfg::BN : 0;
+                    in_x0 = tile_ok && m < args.M;
+                    in_x1 = tile_ok && m + 64 < args.M;
+                    in_w0 = tile_ok;
+                    in_w1 = tile_ok && n + kScaleBlock < args.N;
+                    x0 = args.xs + (in_x0 ? m : 0);
+                    x1 = args.xs + (in_x1 ? m + 64 : 0);
+                    w0 = args.ws + n / kScaleBlock;
+                    w1 = in_w1 ? w0 + 1 : w0;
+                    ahead_left = groups;
+                }
+                float* to = mine + ahead_slot * Cfg::RAW_WORDS;
+                cp_async4(to, x0, in_x0);
+                cp_async4(to + 1, x1, in_x1);
+                cp_async4(to + 2, w0, in_w0);
+                cp_async4(to + 3, w1, in_w1);
+                cp_async_commit();
+                ahead_slot = ahead_slot + 1 == Cfg::RAW_SLOTS ? 0 : ahead_slot + 1;
+                if (--ahead_left > 0) {   // the pointers stop at a tile's last group
+                    x0 += args.xs_stride;
+                    x1 += args.xs_stride;
+                    w0 += args.ws_stride;
+                    w1 += args.ws_stride;
+                }
+            };
+            for (int i = 0; i < Cfg::RAW_SLOTS - 1; ++i) fetch();
+            int slot = 0, s = 0, lag = 0;          // lag: stage of group it - 2
+            uint32_t lag_ph = 0;
+            int it = 0;
             bool ok = true;
             for (int tile = pair; ok && tile < n_tiles; tile += n_pairs) {
-                const int m0 = (tile / tiles_n) * 2 * kTileM + int(rank) * kTileM;
-                const int n0 = (tile % tiles_n) * Cfg::BN + int(rank) * kTileM;
-                for (int g = 0; g < groups; ++g) {
-                    if (!mbar_wait(done + s, ph ^ 1, args.status, kErrTimeoutProducer, abort_flag)) {
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t lfull = mapa_shared(smem_u32(full + s), 0);
-                    if (leader) {
-                        mbar_arrive_expect_tx(full + s, 2 * Cfg::STAGE_BYTES);
-                        armed |= 1u << s;
-                        armed_parity = (armed_parity & ~(1u << s)) | (ph << s);
-                    }
-                    tma_load_2d_pair(sX + s * kHalfBytes, &tmX, lfull, g * kScaleBlock, m0);
-                    tma_load_2d_pair(sW + s * kHalfBytes, &tmW, lfull, g * kScaleBlock, n0);
-                    if (++s == Cfg::STAGES) {
-                        s = 0;
-                        ph ^= 1;
-                    }
-                }
-            }
-            if (!ok && leader) {
-                // Gave up: wait (bounded) for the pair's copies counted on these barriers.
-                for (int i = 0; i < Cfg::STAGES; ++i)
-                    if (armed & (1u << i))
-                        mbar_wait(full + i, (armed_parity >> i) & 1u, args.status, kErrTimeoutDrain, nullptr);
-            }
-        }
-    } else if (warp == 1) {
-        if (leader) {
-            constexpr uint32_t idesc = umma_idesc_e4m3(2 * kTileM, Cfg::BN);
-            const uint64_t dX0 = umma_desc_sw128(smem_u32(sX), 16, 1024);
-            const uint64_t dW0 = umma_desc_sw128(smem_u32(sW), 16, 1024);
-            int s = 0, it = 0;
-            uint32_t ph = 0;
-            bool ok = true, issued = false;
-            for (int tile = pair; ok && tile < n_tiles; tile += n_pairs) {
                 for (int g = 0; g < groups; ++g, ++it) {
-                    const int acc = it & 1;
-                    const uint32_t aph = (it >> 1) & 1;
-                    if (!mbar_wait(full + s, ph, args.status, kErrTimeoutMma, abort_flag) ||
-                        !mbar_wait(tempty + acc, aph ^ 1, args.status, kErrTimeoutMma, abort_flag)) {
-                        ok = false;
-                        break;
+                    fetch();
+                    cp_async_wait<Cfg::RAW_SLOTS - 1>();
+                    const float4 v = *reinterpret_cast<const float4*>(mine + slot * Cfg::RAW_WORDS);
+                    slot = slot + 1 == Cfg::RAW_SLOTS ? 0 : slot + 1;
+                    // Group it - 2 is in its accumulator, so the promotion of group
+                    // it - 4, which this slot held, is over.
+                    if (it >= 2) {
+                        if (!mbar_wait(done + lag, lag_ph, args.status, kErrTimeoutProducer, abort_flag)) {
+                            ok = false;
+                            break;
+                        }
+                        if (++lag == Cfg::STAGES) {
+                            lag = 0;
+                            lag_ph ^= 1;
+                        }
                     }
-                    tc_fence_after();
-                    const uint64_t dx = dX0 + uint64_t(s) * (kHalfBytes >> 4), dw = dW0 + uint64_t(s) * (kHalfBytes >> 4);
-                    if (elect_one()) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            umma_f8_ss_pair(tmem_base + acc * Cfg::BN, dx + 2 * k, dw + 2 * k, idesc, k != 0);
-                        // One commit per group (a second cost 61 clocks of the tensor
-                        // pipe): the stage is free and its sums are in the accumulator.
-                        umma_commit_pair(done + s, 0x3);
-                    }
+                    float* f = factors + (it % Cfg::FACTOR_SLOTS) * Cfg::FACTOR_WORDS + ft;
+                    f[0] = v.x * v.z;
+                    f[64] = v.y * v.z;
+                    f[128] = v.x * v.w;
+                    f[192] = v.y * v.w;
                     __syncwarp();
-                    issued = true;
-                    if (++s == Cfg::STAGES) {
-                        s = 0;
-                        ph ^= 1;
-                    }
+                    if (lane == 0) mbar_arrive(done + s);
+                    s = s + 1 == Cfg::STAGES ? 0 : s + 1;
                 }
             }
-            if (!ok && issued) {
-                if (elect_one()) umma_commit_pair(drain, 0x1);
-                __syncwarp();
-                mbar_wait(drain, 0, args.status, kErrTimeoutDrain, nullptr);
-            }
+            cp_async_wait<0>();
         }
-    } else {
-        // Factor warps: xs ws of this CTA's 128 rows and two weight blocks, for
-        // each group, so that a promotion warp reads one word.  The raw scales
-        // come by cp.async, RAW_SLOTS - 1 groups ahead, into words of the
-        // thread's own.  A group's done barrier counts these warps too.
-        const int ft = int(threadIdx.x) - 64;
-        float* mine = raw + ft * 4;
-        int ahead_tile = pair - n_pairs, ahead_left = 0, ahead_slot = 0;
-        const float *x0 = args.xs, *x1 = args.xs, *w0 = args.ws, *w1 = args.ws;
-        bool in_x0 = false, in_x1 = false, in_w0 = false, in_w1 = false;
-        auto fetch = [&]() {
-            if (ahead_left == 0) {
-                ahead_tile += n_pairs;
-                const bool tile_ok = ahead_tile < n_tiles;
-                const int m = tile_ok ? (ahead_tile / tiles_n) * 2 * kTileM + int(rank) * kTileM + ft : 0;
-                const int n = tile_ok ? (ahead_tile % tiles_n) * Cfg::BN : 0;
-                in_x0 = tile_ok && m < args.M;
-                in_x1 = tile_ok && m + 64 < args.M;
-                in_w0 = tile_ok;
-                in_w1 = tile_ok && n + kScaleBlock < args.N;
-                x0 = args.xs + (in_x0 ? m : 0);
-                x1 = args.xs + (in_x1 ? m + 64 : 0);
-                w0 = args.ws + n / kScaleBlock;
-                w1 = in_w1 ? w0 + 1 : w0;
-                ahead_left = groups;
-            }
-            float* to = mine + ahead_slot * Cfg::RAW_WORDS;
-            cp_async4(to, x0, in_x0);
-            cp_async4(to + 1, x1, in_x1);
-            cp_async4(to + 2, w0, in_w0);
-            cp_async4(to + 3, w1, in_w1);
-            cp_async_commit();
-            ahead_slot = ahead_slot + 1 == Cfg::RAW_SLOTS ? 0 : ahead_slot + 1;
-            if (--ahead_left > 0) {   // the pointers stop at a tile's last group
-                x0 += args.xs_stride;
-                x1 += args.xs_stride;
-                w0 += args.ws_stride;
-                w1 += args.ws_stride;
-            }
-        };
-        for (int i = 0; i < Cfg::RAW_SLOTS - 1; ++i) fetch();
-        int slot = 0, s = 0, lag = 0;          // lag: stage of group it - 2
-        uint32_t lag_ph = 0;
-        int it = 0;
-        bool ok = true;
-        for (int tile = pair; ok && tile < n_tiles; tile += n_pairs) {
-            for (int g = 0; g < groups; ++g, ++it) {
-                fetch();
-                cp_async_wait<Cfg::RAW_SLOTS - 1>();
-                const float4 v = *reinterpret_cast<const float4*>(mine + slot * Cfg::RAW_WORDS);
-                slot = slot + 1 == Cfg::RAW_SLOTS ? 0 : slot + 1;
-                // Group it - 2 is in its accumulator, so the promotion of group
-                // it - 4, which this slot held, is over.
-                if (it >= 2) {
-                    if (!mbar_wait(done + lag, lag_ph, args.status, kErrTimeoutProducer, abort_flag)) {
-                        ok = false;
-                        break;
-                    }
-                    if (++lag == Cfg::STAGES) {
-                        lag = 0;
-                        lag_ph ^= 1;
-                    }
-                }
-                float* f = factors + (it % Cfg::FACTOR_SLOTS) * Cfg::FACTOR_WORDS + ft;
-                f[0] = v.x * v.z;
-                f[64] = v.y * v.z;
-                f[128] = v.x * v.w;
-                f[192] = v.y * v.w;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(done + s);
-                s = s + 1 == Cfg::STAGES ? 0 : s + 1;
-            }
-        }
-        cp_async_wait<0>();
-    }
     } else {
         setmaxnreg_inc<Cfg::MANY_REGS>();
         // Warp w reads TMEM lane quarter w % 4 (rows 32 * (w % 4) .. + 31 of this

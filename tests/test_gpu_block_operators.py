@@ -211,7 +211,8 @@ def test_product_gelu(torch, m, out):
     check_product(torch, x, w, bias, True, out, call_product(torch, x, w, bias, True, out))
 
 
-LARGE = [(2048, 1024, 1024), (2500, 4736, 1024), (5184, 1000, 4736), (4097, 129, 100), (20000, 512, 100), (3000, 257, 4000)]
+LARGE = [(2048, 1024, 1024), (2500, 4736, 1024), (5184, 1000, 4736), (4097, 129, 100), (20000, 512, 100), (3000, 257, 4000),
+         (30011, 11, 500), (9000, 1, 1)]
 
 
 @pytest.mark.parametrize("m, n, k", LARGE)
