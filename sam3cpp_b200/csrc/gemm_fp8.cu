@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(192)
             if (args.gelu) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float2 t = gelu_erf_poly2(make_float2(v[2 * i], v[2 * i + 1]));
+                    const float2 t = gelu_erf_poly2<OUT == kF32>(make_float2(v[2 * i], v[2 * i + 1]));
                     v[2 * i] = t.x;
                     v[2 * i + 1] = t.y;
                 }
@@ -409,7 +409,7 @@ struct PairCfg8 {
     static constexpr int RAW_WORDS = 64 * 4;                   // two row and two block scales per factor thread
     static constexpr int FACTOR_SLOTS = 4;
     static constexpr int FACTOR_WORDS = 2 * kTileM;            // a factor per row and weight block
-    static constexpr uint32_t SMALL_BYTES = 4 * (RAW_SLOTS * RAW_WORDS + FACTOR_SLOTS * FACTOR_WORDS + WARPS * WARP_COLS);
+    static constexpr uint32_t SMALL_BYTES = 4 * (RAW_SLOTS * RAW_WORDS + FACTOR_SLOTS * FACTOR_WORDS + 2 * WARPS * WARP_COLS);
     static constexpr uint32_t TMEM_COLS = 2 * BN;
     static constexpr size_t SMEM = RING + OUT_BYTES + SMALL_BYTES + 1024 + 256;
     // Warpgroup 0: TMA producer, UMMA issuer and two factor warps; warpgroups 1
@@ -435,7 +435,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
     float* raw = reinterpret_cast<float*>(sOut + Cfg::OUT_BYTES);
     float* factors = raw + Cfg::RAW_SLOTS * Cfg::RAW_WORDS;
     float* biases = factors + Cfg::FACTOR_SLOTS * Cfg::FACTOR_WORDS;
-    uint64_t* full = reinterpret_cast<uint64_t*>(biases + Cfg::WARPS * Cfg::WARP_COLS);
+    uint64_t* full = reinterpret_cast<uint64_t*>(biases + 2 * Cfg::WARPS * Cfg::WARP_COLS);
     uint64_t* done = full + Cfg::STAGES;
     uint64_t* tempty = done + Cfg::STAGES;
     uint64_t* drain = tempty + 2;
@@ -628,26 +628,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         const uint32_t lanes = uint32_t(quarter * 32) << 16;
         uint8_t* stage = sOut + (warp - 4) * Cfg::OUT_BUFS * Cfg::OUT_BUF;
-        float* my_bias = biases + (warp - 4) * Cfg::WARP_COLS;
+        float* my_bias = biases + (warp - 4) * 2 * Cfg::WARP_COLS;   // this tile's and the next one's
         const uint32_t my_factor = smem_u32(factors + half * kTileM + quarter * 32 + lane);
         int it = 0, out = 0, s = 0;   // groups promoted, the next buffer of y, the group's stage
         uint32_t ph = 0;
         bool ok = true;
+        auto fetch_bias = [&](int tile, int which) {
+            const int n0 = (tile % tiles_n) * Cfg::BN + half * Cfg::WARP_COLS;
+#pragma unroll
+            for (int i = 0; i < Cfg::WARP_COLS / 32; ++i) {
+                const int n = n0 + lane + 32 * i;
+                const bool take = tile < n_tiles && n < args.N;
+                cp_async4(my_bias + which * Cfg::WARP_COLS + lane + 32 * i, args.bias + (take ? n : 0), take);
+            }
+            cp_async_commit();
+        };
+        int which = 0;
+        if (args.bias) fetch_bias(pair, 0);
         for (int tile = pair; ok && tile < n_tiles; tile += n_pairs) {
             const int row0 = (tile / tiles_n) * 2 * kTileM + int(rank) * kTileM + quarter * 32;
             const int n0 = (tile % tiles_n) * Cfg::BN + half * Cfg::WARP_COLS;
-            if (args.bias) {   // for the epilogue
+            // The sums begin with the bias, which came during the tile before.
+            float2 sum[Cfg::WARP_COLS / 2];
+            if (args.bias) {
+                cp_async_wait<0>();
                 __syncwarp();
 #pragma unroll
-                for (int i = 0; i < Cfg::WARP_COLS / 32; ++i) {
-                    const int n = n0 + lane + 32 * i;
-                    cp_async4(my_bias + lane + 32 * i, args.bias + (n < args.N ? n : 0), n < args.N);
+                for (int i = 0; i < Cfg::WARP_COLS / 4; ++i) {
+                    const float4 b = ld_shared_f4(smem_u32(my_bias) + which * Cfg::WARP_COLS * 4 + 16 * i);
+                    sum[2 * i] = make_float2(b.x, b.y);
+                    sum[2 * i + 1] = make_float2(b.z, b.w);
                 }
-                cp_async_commit();
-            }
-            float2 sum[Cfg::WARP_COLS / 2];
+                which ^= 1;
+                fetch_bias(tile + n_pairs, which);   // every lane left that buffer a tile ago
+            } else {
 #pragma unroll
-            for (int i = 0; i < Cfg::WARP_COLS / 2; ++i) sum[i] = make_float2(0.f, 0.f);
+                for (int i = 0; i < Cfg::WARP_COLS / 2; ++i) sum[i] = make_float2(0.f, 0.f);
+            }
             // 64 columns on their way at a time, across groups too: the next
             // group's first columns are asked for before the last of this one
             // are added.  The accumulator goes back to the UMMA issuer once its
@@ -705,24 +722,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
             }
             if (!ok) break;
             if (n0 >= args.N || row0 >= args.M) continue;   // warp-uniform: nothing of y here
-            if (args.bias) {
-                cp_async_wait<0>();   // issued a tile ago
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < Cfg::WARP_COLS / 4; i += 8) {
-                    float4 b[8];
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) b[k] = ld_shared_f4(smem_u32(my_bias) + 16 * (i + k));
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        sum[2 * (i + k)] = __fadd2_rn(sum[2 * (i + k)], make_float2(b[k].x, b[k].y));
-                        sum[2 * (i + k) + 1] = __fadd2_rn(sum[2 * (i + k) + 1], make_float2(b[k].z, b[k].w));
-                    }
-                }
-            }
             if (args.gelu) {
 #pragma unroll
-                for (int i = 0; i < Cfg::WARP_COLS / 2; ++i) sum[i] = gelu_erf_poly2(sum[i]);
+                for (int i = 0; i < Cfg::WARP_COLS / 2; ++i) sum[i] = gelu_erf_poly2<OUT == kF32>(sum[i]);
             }
             // Each lane writes 128 bytes of its row at a time to a swizzled stage,
             // and one TMA store per warp takes the 32 rows while the next tile is
@@ -791,6 +793,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
                 if (lane == 0) bulk_commit_group();   // one group a chunk, empty where the warp copied
             }
         }
+        cp_async_wait<0>();
         if (lane == 0) bulk_wait_group_all();
     }
 

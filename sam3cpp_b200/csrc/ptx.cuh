@@ -587,29 +587,34 @@ S3T_DEV float2 gelu_erf_as2(float2 x) {
     return __ffma2_rn(u, e, make_float2(fmaxf(x.x, 0.f), fmaxf(x.y, 0.f)));
 }
 
-// Two lanes of GELU with one 2^x each and no reciprocal: GELU(x) = relu(x) -
-// a Q(a), a = |x|, Q(a) = erfc(a / sqrt 2) / 2 = 2^P(a), where P is a degree 7
-// polynomial fitted here to log2 Q on [0, 6] (weighted minimax; the error of
-// a Q stays below 1.5e-7 and below 6.5e-8 a, and 2^x adds 2^-22 of a Q).
-// Beyond 6, a Q is below 6e-9 and held there.  The epilogue that uses it has
-// the special-function unit as its bound: 4096 clocks a 128 x 256 tile with
-// two such operations an element.
+// The larger of two, NaN if one is NaN.
 S3T_DEV float max_nan(float a, float b) {
     float d;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
 
+// Two lanes of GELU with one 2^x each and no reciprocal: GELU(x) = relu(x) -
+// a Q(a), a = |x|, Q(a) = erfc(a / sqrt 2) / 2 = 2^P(a), where P is a
+// polynomial fitted here to log2 Q on [0, 6] (minimax weighted by Q): degree 7
+// (FINE), an error of a Q below 6.5e-8 a, for fp32 results, or degree 5, below
+// 3.2e-7 a, where the result is rounded to 16 or 8 bits.  2^x adds 2^-22 of
+// a Q.  Beyond 6, a Q is below 6e-9 and held there.
+template <bool FINE>
 S3T_DEV float2 gelu_erf_poly2(float2 x) {
+    constexpr float kFine[8] = {-9.9999988079071045e-01f, -1.1511108875274658f,     -4.591531455516815e-01f,
+                                -5.269110947847366e-02f,  7.389270234853029e-03f,   -4.212349303998053e-04f,
+                                -5.390396108850837e-05f,  8.470184184261598e-06f};
+    constexpr float kCoarse[6] = {-1.0000008344650269f,    -1.1510831117630005f,   -4.592766761779785e-01f,
+                                  -5.253801867365837e-02f, 7.387201767414808e-03f, -5.188587820157409e-04f};
+    constexpr int DEG = FINE ? 7 : 5;
     const float2 a = make_float2(fminf(fabsf(x.x), 6.f), fminf(fabsf(x.y), 6.f));
-    float2 p = make_float2(8.470184184261598e-06f, 8.470184184261598e-06f);
-    p = __ffma2_rn(p, a, make_float2(-5.390396108850837e-05f, -5.390396108850837e-05f));
-    p = __ffma2_rn(p, a, make_float2(-4.212349303998053e-04f, -4.212349303998053e-04f));
-    p = __ffma2_rn(p, a, make_float2(7.389270234853029e-03f, 7.389270234853029e-03f));
-    p = __ffma2_rn(p, a, make_float2(-5.269110947847366e-02f, -5.269110947847366e-02f));
-    p = __ffma2_rn(p, a, make_float2(-4.591531455516815e-01f, -4.591531455516815e-01f));
-    p = __ffma2_rn(p, a, make_float2(-1.1511108875274658f, -1.1511108875274658f));
-    p = __ffma2_rn(p, a, make_float2(-9.9999988079071045e-01f, -9.9999988079071045e-01f));
+    float2 p = make_float2(FINE ? kFine[7] : kCoarse[5], FINE ? kFine[7] : kCoarse[5]);
+#pragma unroll
+    for (int k = DEG - 1; k >= 0; --k) {
+        const float c = FINE ? kFine[k] : kCoarse[FINE ? 0 : k];
+        p = __ffma2_rn(p, a, make_float2(c, c));
+    }
     const float2 q = make_float2(ex2_approx(p.x), ex2_approx(p.y));
     return __ffma2_rn(make_float2(-a.x, -a.y), q, make_float2(max_nan(x.x, 0.f), max_nan(x.y, 0.f)));
 }
