@@ -43,6 +43,7 @@ constexpr int kSlots = 1;              // rows ahead of a warp (STREAM)
 constexpr int kStreamWarps = 16;
 constexpr int kStreamBytes = 200 * 1024;
 constexpr int kVectors = 5;            // post weight and bias, branch factor, pre weight and bias
+constexpr int kStreamVectors = 4;      // the branch factor folded into the first two
 
 // A lane's eight elements of a chunk are two quads: quad h is columns
 // h * 128 + 4 lane .. + 3 (VEC: whole or not there at all), or h * 128 + lane +
@@ -242,7 +243,8 @@ S3T_DEV void store_eight(const NormResidualArgs& a, uint32_t row, int c0, int la
 #pragma unroll
     for (int k = 0; k < 2 * CPW; ++k) {
         const float2 p = v[k / 2][2 * (k & 1)], q = v[k / 2][2 * (k & 1) + 1];
-        peak[k] = __reduce_max_sync(0xffffffffu, max(max(abs_bits(p.x), abs_bits(p.y)), max(abs_bits(q.x), abs_bits(q.y))));
+        // The bits of magnitudes order like them, NaN above all (and kept by absmax3_nan).
+        peak[k] = __reduce_max_sync(0xffffffffu, abs_bits(absmax3_nan(absmax3_nan(p.x, p.y, q.x), q.y, q.y)));
     }
     // Lane 2 k divides for group k's scale, lane 2 k + 1 for its inverse.
     uint32_t pick = peak[0];
@@ -355,15 +357,12 @@ struct StreamRow {
     static constexpr uint32_t BYTES = X + 2 * Y;
 };
 
-// The 16-byte units that hold `bytes` bytes from p on; returns their size.
-S3T_DEV uint32_t bulk_load_around(uint8_t* to, const void* p, uint32_t bytes, uint64_t* bar) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(p), first = at & ~uintptr_t(15);
-    const uint32_t size = (uint32_t(at - first) + bytes + 15) & ~15u;
-    bulk_load(to, reinterpret_cast<const void*>(first), size, bar);
-    return size;
-}
+// The 16-byte units that hold `bytes` bytes from p on.
 S3T_DEV uint32_t units_around(const void* p, uint32_t bytes) {
     return ((uint32_t(reinterpret_cast<uintptr_t>(p)) & 15) + bytes + 15) & ~15u;
+}
+S3T_DEV void bulk_load_around(uint8_t* to, const void* p, uint32_t bytes, uint64_t* bar) {
+    bulk_load(to, reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(15)), units_around(p, bytes), bar);
 }
 
 // VEC: rows and columns in whole 16-byte units; else the units around a row
@@ -382,16 +381,19 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
     const int c0 = warp * int(Row::COLS), cols = warp + 1 == warps ? last : int(Row::COLS);
     float* vec = reinterpret_cast<float*>(words);
     {
-        const float* const from[kVectors] = {a.post_weight, a.post_bias, a.channel, a.pre_weight, a.pre_bias};
-#pragma unroll
-        for (int k = 0; k < kVectors; ++k) {
-            const float otherwise = k == 1 || k == 4 ? 0.f : 1.f, times = k == 2 ? a.branch_scale : 1.f;
-            for (int c = thread; c < padded; c += threads)
-                vec[k * padded + c] = c < dim ? (from[k] ? from[k][c] : otherwise) * times : 0.f;
+        // Weight and bias of the branch with its scales folded in (the bias only
+        // with a post-norm), then those of the pre-norm; 0 past dim.
+        for (int c = thread; c < padded; c += threads) {
+            const bool in = c < dim;
+            const float s = in ? a.branch_scale * (a.channel ? a.channel[c] : 1.f) : 0.f;
+            vec[c] = a.post && a.post_weight && in ? a.post_weight[c] * s : s;
+            vec[padded + c] = a.post && a.post_bias && in ? a.post_bias[c] * s : 0.f;
+            vec[2 * padded + c] = in ? (a.pre_weight ? a.pre_weight[c] : 1.f) : 0.f;
+            vec[3 * padded + c] = a.pre_bias && in ? a.pre_bias[c] : 0.f;
         }
     }
     // VEC: columns past dim are never copied, they stay zeros.
-    uint8_t* mine = reinterpret_cast<uint8_t*>(vec + kVectors * padded) + (team * warps + warp) * kSlots * Row::BYTES;
+    uint8_t* mine = reinterpret_cast<uint8_t*>(vec + kStreamVectors * padded) + (team * warps + warp) * kSlots * Row::BYTES;
     for (uint32_t i = lane; i < kSlots * Row::BYTES / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
     uint64_t* bar = arrived[team * warps + warp];
     if (lane == 0) {
@@ -415,11 +417,18 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
         const uint32_t xb = uint32_t(cols) * sizeof(R), tb = uint32_t(cols) * sizeof(T);
         const T* gp = static_cast<const T*>(a.gate);
         if (a.gate) gp += int64_t(ahead / uint32_t(a.gate_rows)) * a.gate_stride + c0;
-        mbar_arrive_expect_tx(bar + slot, units_around(xp, xb) + (a.y ? units_around(yp, tb) : 0) +
-                                              (a.gate ? units_around(gp, tb) : 0));
-        if (a.y) bulk_load_around(to + Row::X, yp, tb, bar + slot);
-        bulk_load_around(to, xp, xb, bar + slot);
-        if (a.gate) bulk_load_around(to + Row::X + Row::Y, gp, tb, bar + slot);
+        if constexpr (VEC) {
+            mbar_arrive_expect_tx(bar + slot, xb + (a.y ? tb : 0) + (a.gate ? tb : 0));
+            if (a.y) bulk_load(to + Row::X, yp, tb, bar + slot);
+            bulk_load(to, xp, xb, bar + slot);
+            if (a.gate) bulk_load(to + Row::X + Row::Y, gp, tb, bar + slot);
+        } else {
+            mbar_arrive_expect_tx(bar + slot, units_around(xp, xb) + (a.y ? units_around(yp, tb) : 0) +
+                                                  (a.gate ? units_around(gp, tb) : 0));
+            if (a.y) bulk_load_around(to + Row::X, yp, tb, bar + slot);
+            bulk_load_around(to, xp, xb, bar + slot);
+            if (a.gate) bulk_load_around(to + Row::X + Row::Y, gp, tb, bar + slot);
+        }
         xp += x_step;
         yp += y_step;
         ahead = rows - ahead > stride ? ahead + stride : rows;
@@ -455,6 +464,14 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
                     vector(1, j, b);
                     normalize(h[j], st, w, b);
                 }
+            } else {
+#pragma unroll
+                for (int j = 0; j < CPW; ++j) {
+                    float2 w[4];
+                    vector(0, j, w);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) h[j][i] = __fmul2_rn(h[j][i], w[i]);
+                }
             }
             if (a.gate) {
 #pragma unroll
@@ -470,10 +487,8 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
         for (int j = 0; j < CPW; ++j) {
             chunk(from, static_cast<const R*>(a.x) + int64_t(row) * a.x_stride + c0, j, x[j]);
             if (a.y) {
-                float2 s[4];
-                vector(2, j, s);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[j][i] = __ffma2_rn(both(a.resid_scale), x[j][i], __fmul2_rn(s[i], h[j][i]));
+                for (int i = 0; i < 4; ++i) x[j][i] = __ffma2_rn(both(a.resid_scale), x[j][i], h[j][i]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[j][i] = __fmul2_rn(both(a.resid_scale), x[j][i]);
@@ -493,8 +508,8 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
 #pragma unroll
             for (int j = 0; j < CPW; ++j) {
                 float2 w[4], b[4];
-                vector(3, j, w);
-                vector(4, j, b);
+                vector(2, j, w);
+                vector(3, j, b);
                 normalize(x[j], st, w, b);
                 if (!a.u_eight)
                     store_chunk<VEC>(static_cast<T*>(a.u) + int64_t(row) * a.u_stride, c0 + j * kChunk, dim, lane, x[j]);
@@ -520,7 +535,7 @@ template <typename T, typename R, int CPW>
 bool launch_stream(const NormResidualArgs& a, int num_sms, cudaStream_t stream) {
     using Row = StreamRow<T, R, CPW>;
     const int warps = (a.dim + int(Row::COLS) - 1) / int(Row::COLS);
-    const int vector_bytes = kVectors * warps * int(Row::COLS) * 4;
+    const int vector_bytes = kStreamVectors * warps * int(Row::COLS) * 4;
     int teams = vector_bytes < kStreamBytes ? (kStreamBytes - vector_bytes) / (warps * kSlots * int(Row::BYTES)) : 0;
     if (teams > kStreamWarps / warps) teams = kStreamWarps / warps;
     // Two rows a team and more: the rows ahead pay for the set-up.
