@@ -14,13 +14,16 @@
 // reduction); warp w of a row's team holds CPW consecutive chunks.
 //
 // Many rows (STREAM): persistent CTAs, up to four chunks a warp, so that a
-// reduction or a barrier is paid once for 32 columns a lane; the vectors wait in shared
-// memory and the next row comes there by bulk copies while the second half of
-// a row is computed.  82944 x 1024, LayerNorm twice, gate, e4m3 out: 155 us,
-// 6.0 TB/s with 16 warps an SM and one row ahead (12 warps and two rows: 174
-// us, 20 warps of fewer registers: 168 us); whole rows per warp read straight
-// into registers took 398 us (the loads' latency), one chunk a warp with the
-// next row in registers 269 us (four times the reductions).
+// reduction or a barrier is paid once for 32 columns a lane; the vectors wait in
+// shared memory (the branch's scales folded into the post-norm's: one multiply
+// less a value) and the next row comes there by bulk copies while the second
+// half of a row is computed.  82944 x 1024, LayerNorm twice, gate, e4m3 out:
+// 155-162 us, 5.8-6.0 TB/s with 16 warps an SM and one row ahead (12 warps and
+// two rows: 174 us, 20 warps of fewer registers: 168 us); in runs of seconds
+// under the 1 kW cap 172 us, where instructions count (178 us with 5% more).
+// Whole rows per warp read straight into registers took 398 us (the loads'
+// latency), one chunk a warp with the next row in registers 269 us (four times
+// the reductions).
 // Few rows: one chunk a warp up to 4096 columns, everything asked for at once,
 // for the latency of one row.
 //
@@ -439,9 +442,13 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
     bool lost = false;
     for (uint32_t it = 0; row < rows; ++it) {
         const int slot = int(it % kSlots);
-        // A row that never came is reported; the loop goes on without waiting, so
-        // that no warp of the team is left alone at a barrier.
-        lost = lost || !mbar_wait(bar + slot, (it / kSlots) & 1, a.status, kErrTimeoutProducer, nullptr);
+        // A row that never came is reported and no more are asked for; the loop
+        // goes on without waiting, so that no warp of the team is left alone at a
+        // barrier, and the copy has a second limit's time before the CTA may end.
+        if (!lost && !mbar_wait(bar + slot, (it / kSlots) & 1, a.status, kErrTimeoutProducer, nullptr)) {
+            lost = true;
+            mbar_wait(bar + slot, (it / kSlots) & 1, a.status, kErrTimeoutDrain, nullptr);
+        }
         const uint8_t* from = mine + slot * Row::BYTES;
         float2 x[CPW][4], h[CPW][4];
         auto vector = [&](int k, int j, float2(&v)[4]) { load_chunk<VEC>(vec + k * padded + c0 + j * kChunk, 0, kChunk, lane, v); };
@@ -495,7 +502,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
             }
         }
         __syncwarp();
-        if (lane == 0) fetch(slot);   // every lane has read the slot
+        if (lane == 0 && !lost) fetch(slot);   // every lane has read the slot
         if (a.x_out) {
 #pragma unroll
             for (int j = 0; j < CPW; ++j) {

@@ -597,9 +597,10 @@ S3T_DEV float max_nan(float a, float b) {
 // Two lanes of GELU with one 2^x each and no reciprocal: GELU(x) = relu(x) -
 // a Q(a), a = |x|, Q(a) = erfc(a / sqrt 2) / 2 = 2^P(a), where P is a
 // polynomial fitted here to log2 Q on [0, 6] (minimax weighted by Q): degree 7
-// (FINE), an error of a Q below 6.5e-8 a, for fp32 results, or degree 5, below
-// 3.2e-7 a, where the result is rounded to 16 or 8 bits.  2^x adds 2^-22 of
-// a Q.  Beyond 6, a Q is below 6e-9 and held there.
+// (FINE), an error of a Q below 6.5e-8 a, which is what fp32 arithmetic leaves
+// of (1 + erf) / 2; or degree 5, below 3.2e-7 a, for results that share an
+// 8-bit block's scale (half a step near zero: 2.2e-6 of its largest).  2^x adds
+// 2^-22 of a Q.  Beyond 6, a Q is below 6e-9 and held there.
 template <bool FINE>
 S3T_DEV float2 gelu_erf_poly2(float2 x) {
     constexpr float kFine[8] = {-9.9999988079071045e-01f, -1.1511108875274658f,     -4.591531455516815e-01f,

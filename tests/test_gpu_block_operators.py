@@ -211,6 +211,40 @@ def test_product_gelu(torch, m, out):
     check_product(torch, x, w, bias, True, out, call_product(torch, x, w, bias, True, out))
 
 
+@pytest.mark.parametrize("m", [3, 100, 2600])
+@pytest.mark.parametrize("out", ["f32", "f16", "bf16", "e4m3"])
+def test_product_gelu_by_its_argument(torch, m, out):
+    """Zero products: y is GELU(bias), from the flat tail to the linear end.  The kernel takes |b| to at most 6 and
+    Q = erfc(|b| / sqrt 2) / 2 as 2^P: a polynomial within 6.5e-8 of Q (8 bits: 3.2e-7), eight roundings of partial sums
+    no larger than 1 + |P|, a 2^x within 2^-22 and the rounding of the last sum."""
+    n = 640
+    x, w = Eight(torch, m, 130), Eight(torch, n, 130, 128)
+    for t in (x, w):
+        t.q[:] = 0
+        t.scale[:] = 1
+    b = torch.linspace(-8, 8, n, device="cuda")
+    if out != "e4m3":
+        b[[0, 1, 2]] = torch.tensor([float("nan"), float("inf"), -float("inf")], device="cuda")
+        b[[3, 4, 5]] = torch.tensor([3e4, -3e4, -0.0], device="cuda")
+    y = call_product(torch, x, w, b, True, out)
+    if out != "e4m3":
+        assert torch.isnan(y[:m, 0]).all() and (y[:m, 1] == float("inf")).all() and (y[:m, 2].abs() < 1e-8).all()
+        b[[0, 1, 2]] = 1.0
+    v = b.double()
+    a, q = v.abs().clamp(max=6), torch.special.erfc(v.abs().clamp(max=6) * math.sqrt(0.5)) / 2
+    want = 0.5 * v * torch.special.erfc(-v * math.sqrt(0.5))
+    poly = 3.2e-7 if out == "e4m3" else 6.5e-8
+    e = a * (poly + q * (2.0 ** -22 + 2.0 ** -21 * (1 + q.log2().abs()))) + want.abs() * U + 6e-9
+    if out == "e4m3":
+        err = (y.values(torch) - want).abs()
+        assert (err <= (want.abs() + e) * (2.0 ** -4 + 4 * U) + y.spans() * 2.0 ** -10 + e).all()
+        return
+    got = y[:m].double()
+    err = (got - want).abs()[:, 3:]
+    half, tiny = KINDS[out][2], 2.0 ** -25 if out == "f16" else 0.0
+    assert (err <= (e + (want.abs() + e) * half + tiny)[3:]).all(), float((err - e[3:]).max())
+
+
 LARGE = [(2048, 1024, 1024), (2500, 4736, 1024), (5184, 1000, 4736), (4097, 129, 100), (20000, 512, 100), (3000, 257, 4000),
          (30011, 11, 500), (9000, 1, 1)]
 
