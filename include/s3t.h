@@ -267,7 +267,7 @@ int s3t_layernorm(int device, const float *x, int rows, const float *gamma, cons
  * Strides count elements.  Inputs are read in whole 16-byte units that hold one
  * of their bytes.  Outputs overlap no input, except where in place is allowed
  * below.  A call with no rows or tokens (or no columns) writes nothing
- * and succeeds. */
+ * and succeeds, whatever its pointers and strides. */
 
 /* Rows of a matrix in device memory.  scale and scale_stride belong to e4m3
  * matrices: the scale of column group g (128 columns; the last may be

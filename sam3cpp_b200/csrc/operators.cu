@@ -82,12 +82,12 @@ int s3t_quantize_fp8(int device, int type, const void* x, int64_t rows, int64_t 
         if (kind < 0 || kind == kE4M3) return refuse(op, "x must be F32, F16 or BF16");
         if (rows < 0 || cols < 0) return refuse(op, "rows and cols must not be negative");
         if (block_rows != 1 && block_rows != kScaleBlock) return refuse(op, "block_rows must be 1 or 128");
+        if (rows == 0 || cols == 0) return 0;   // the arrays may be null: empty tensors are
         if (!x || !aligned(x, element_bytes(kind))) return refuse(op, "x must be a device pointer aligned to its type");
         if (x_stride < cols) return refuse(op, "x_stride is below cols");
         if (const char* why = bad_eight(q, cols, block_rows == 1 ? rows : blocks(rows))) return refuse(op, why);
         // Far beyond any GPU's memory; keeps every offset inside 64 bits.
         if (rows > (int64_t(1) << 40) || cols > (int64_t(1) << 40)) return refuse(op, "rows or cols too large");
-        if (rows == 0 || cols == 0) return 0;
         QuantizeArgs a{};
         a.x = x;
         a.rows = rows; a.cols = cols; a.x_stride = x_stride;
@@ -111,6 +111,7 @@ int s3t_gemm_fp8(int device, const s3t_matrix* x, const s3t_matrix* w, const flo
         if (M < 0 || N < 0 || K < 1) return refuse(op, "needs M >= 0, N >= 0 and K >= 1");
         if (M > kMost || N > kMost || K > kMost) return refuse(op, "M, N and K must be at most 2^30");
         if (act != 0 && act != 1) return refuse(op, "act must be 0 (none) or 1 (GELU)");
+        if (M == 0 || N == 0) return 0;
         if (const char* why = bad_eight(x, K, M)) return refuse(op, std::string("x: ") + why);
         if (const char* why = bad_eight(w, K, blocks(N))) return refuse(op, std::string("w: ") + why);
         if (!aligned(bias, 4)) return refuse(op, "bias must be 4-byte aligned");
@@ -121,7 +122,6 @@ int s3t_gemm_fp8(int device, const s3t_matrix* x, const s3t_matrix* w, const flo
                 return refuse(op, "y must be a device pointer aligned to its type");
             if (y->stride < N) return refuse(op, "the row stride of y is below N");
         }
-        if (M == 0 || N == 0) return 0;
         GemmFp8Args a{};
         a.M = M; a.N = N; a.K = K;
         a.x = static_cast<const uint8_t*>(x->data);
@@ -160,8 +160,9 @@ int s3t_norm_residual(int device, const s3t_norm_args* p, void* stream) {
             return refuse(op, "unknown flags");
         const bool sigmoid = p->flags & S3T_NORM_GATE_SIGMOID, tanh = p->flags & S3T_NORM_GATE_TANH;
         if (sigmoid && tanh) return refuse(op, "a gate is a sigmoid or a tanh, not both");
-        if ((sigmoid || tanh) && !p->gate) return refuse(op, "a gate function needs the gate array");
         if (!(p->eps >= 0.f) || !std::isfinite(p->eps)) return refuse(op, "eps must be finite and not negative");
+        if (p->rows == 0) return 0;
+        if ((sigmoid || tanh) && !p->gate) return refuse(op, "a gate function needs the gate array");
         const int eb = element_bytes(kind), rb = element_bytes(resid), dim = p->dim;
         if (!p->x || !aligned(p->x, rb) || p->x_stride < dim) return refuse(op, "x must be an aligned device pointer with x_stride >= dim");
         if (!p->y && (p->gate || p->channel_scale || (p->flags & S3T_NORM_POST)))
@@ -192,7 +193,6 @@ int s3t_norm_residual(int device, const s3t_norm_args* p, void* stream) {
         }
         vec = vec && (!p->y || rows16(p->y, p->y_stride, kind)) && (!p->gate || rows16(p->gate, p->gate_stride, kind)) &&
               (!p->x_out || rows16(p->x_out, p->x_out_stride, resid));
-        if (p->rows == 0) return 0;
         NormResidualArgs a{};
         a.rows = p->rows; a.dim = dim;
         a.kind = kind; a.resid_kind = resid;
@@ -260,6 +260,7 @@ int s3t_rotary(int device, const double* freq, int rot_dim, float magnitude, con
         if (rot_dim < 2 || rot_dim > head_dim || rot_dim % 2) return refuse(op, "rot_dim must be even and in [2, head_dim]");
         if (flags & ~(S3T_ROTARY_INTERLEAVED | S3T_ROTARY_INVERSE)) return refuse(op, "unknown flags");
         if (tokens < 0 || tokens > (int64_t(1) << 31) - 1) return refuse(op, "tokens must be in [0, 2^31)");
+        if (tokens == 0) return 0;
         if (!freq || !aligned(freq, 8)) return refuse(op, "freq must be an aligned device pointer");
         if (!positions || !aligned(positions, 8)) return refuse(op, "positions must be an aligned device pointer");
         if (!q) return refuse(op, "q must not be null");
@@ -291,7 +292,6 @@ int s3t_rotary(int device, const double* freq, int rot_dim, float magnitude, con
             marks |= uint64_t(p.x_token) | uint64_t(p.x_head) | uint64_t(p.out_token) | uint64_t(p.out_head);
         }
         a.run = marks % uint64_t(16 / eb) == 0 ? 16 / eb : marks % 2 == 0 ? 2 : 1;
-        if (tokens == 0) return 0;
         a.freq = freq;
         a.rot = rot_dim;
         a.magnitude = magnitude;

@@ -160,6 +160,30 @@ def test_empty_calls_succeed_without_a_device():
     s3t.rotary(0, A, 32, 1.0, A, 0, a["type"], 64, a["q"])
 
 
+def test_empty_calls_take_the_null_pointers_of_empty_tensors():
+    none = s3t.Matrix(None, 256, None, 256)
+    for kind in (s3t.TYPE_F32, s3t.TYPE_BF16):
+        s3t.quantize_fp8(0, kind, None, 0, 200, 200, 1, none)
+        s3t.quantize_fp8(0, kind, None, 5, 0, 0, 1, none)
+    for y_type in (s3t.TYPE_F32, s3t.TYPE_E4M3):
+        s3t.gemm_fp8(0, none, eight(), A, 0, 200, 200, 1, y_type, none)
+        s3t.gemm_fp8(0, eight(), none, None, 5, 0, 200, 0, y_type, none)
+    empty = dict(rows=0, x=None, y=None, gate=None, x_out=None, u=none)
+    s3t.norm_residual(0, s3t.NormArgs(**{**NORM, **empty}))
+    s3t.norm_residual(0, s3t.NormArgs(**{**NORM, **empty, "flags": s3t.NORM_POST | s3t.NORM_GATE_TANH, "u_type": s3t.TYPE_E4M3}))
+    v = s3t.RotaryView(None, None, 4, 256, 64, 256, 64)
+    s3t.rotary(0, A, 32, 1.0, None, 0, s3t.TYPE_F16, 64, v, v)
+    # what does not depend on the pointers is refused all the same
+    with refused("block_rows"):
+        s3t.quantize_fp8(0, s3t.TYPE_F32, None, 0, 200, 200, 64, none)
+    with refused("act"):
+        s3t.gemm_fp8(0, none, eight(), None, 0, 200, 200, 7, s3t.TYPE_F32, none)
+    with refused("eps"):
+        s3t.norm_residual(0, s3t.NormArgs(**{**NORM, **empty, "eps": -1.0}))
+    with refused("rot_dim"):
+        s3t.rotary(0, A, 31, 1.0, None, 0, s3t.TYPE_F16, 64, v)
+
+
 def test_a_call_without_a_gpu_is_an_error():
     import torch
     if torch.cuda.is_available():
