@@ -17,9 +17,9 @@
 // pipe and the promotion together: the accumulators fill tensor memory, two
 // groups are in flight, and a group's accumulator is free again about 700
 // clocks after it is full.  A tile's epilogue is not overlapped with the next
-// mainloop beyond those two groups (2000 clocks for fp16, 4000 with GELU and
-// e4m3), which is what K = 1024 pays for: 5184 x 4736 x 1024, GELU, e4m3 43-48
-// us.
+// mainloop beyond those two groups (2700 clocks for fp16, 5000 with GELU and
+// e4m3, when the bias was still added there; now it begins the sums), which is
+// what K = 1024 pays for: 5184 x 4736 x 1024, GELU, e4m3 43-48 us.
 //
 // gemm_fp8_tile_kernel: for few rows, with the operands swapped: 128 rows of w
 // are the UMMA's M and 16 to 64 rows of x its N, so one token costs one pass
