@@ -27,6 +27,8 @@
 // Few rows: one chunk a warp up to 4096 columns, everything asked for at once,
 // for the latency of one row.
 //
+// Up to 128 columns: several rows a warp (norm_narrow_kernel).
+//
 // A LayerNorm warp reduces its own mean and centred square sum and the warps'
 // are merged about the row's mean (Chan, Golub and LeVeque, 1979), so there is
 // one exchange per norm and no cancellation.
@@ -44,6 +46,7 @@ constexpr int kChunk = 2 * kScaleBlock;
 constexpr int kMaxWarps = 16;          // of a team: 16 x 4 chunks hold kNormMaxDim columns
 constexpr int kSlots = 1;              // rows ahead of a warp (STREAM)
 constexpr int kStreamWarps = 16;
+constexpr int kNarrowThreads = 256;
 constexpr int kStreamBytes = 200 * 1024;
 constexpr int kVectors = 5;            // post weight and bias, branch factor, pre weight and bias
 constexpr int kStreamVectors = 4;      // the branch factor folded into the first two
@@ -528,6 +531,226 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
     }
 }
 
+// ------------------------------------------------------- rows up to 128 ---
+
+// Columns of element i of a lane's eight, LANES lanes a row.
+template <int LANES, bool VEC>
+S3T_DEV int narrow_col(int l, int i) {
+    return VEC ? l * 8 + i : l + LANES * i;
+}
+
+// A lane's elements as they lie in memory: widened where they are used, since
+// a conversion would wait for the load.
+template <typename T>
+struct alignas(16) NarrowRaw {
+    T e[8];
+};
+
+template <int LANES, bool VEC, typename T>
+S3T_DEV void narrow_load(const T* p, int dim, int l, bool there, NarrowRaw<T>& v) {
+    if constexpr (VEC) {
+        uint4 u[sizeof(T) / 2];
+#pragma unroll
+        for (int i = 0; i < int(sizeof(T)) / 2; ++i)
+            u[i] = there && l * 8 < dim ? reinterpret_cast<const uint4*>(p + l * 8)[i] : make_uint4(0, 0, 0, 0);
+        memcpy(v.e, u, sizeof(u));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int c = narrow_col<LANES, false>(l, i);
+            v.e[i] = there && c < dim ? p[c] : from_float<T>(0.f);
+        }
+    }
+}
+
+template <typename T>
+S3T_DEV void narrow_widen(const NarrowRaw<T>& r, float2 (&v)[4]) {
+    widen4(r.e, v[0], v[1]);
+    widen4(r.e + 4, v[2], v[3]);
+}
+
+template <int LANES, bool VEC, typename T>
+S3T_DEV void narrow_store(T* p, int dim, int l, const float2 (&v)[4]) {
+    if constexpr (VEC) {
+        if (l * 8 >= dim) return;
+        if constexpr (sizeof(T) == 4) {
+            reinterpret_cast<float4*>(p + l * 8)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+            reinterpret_cast<float4*>(p + l * 8)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+        } else {
+            *reinterpret_cast<uint4*>(p + l * 8) = make_uint4(pack2(v[0].x, v[0].y, T()), pack2(v[1].x, v[1].y, T()),
+                                                              pack2(v[2].x, v[2].y, T()), pack2(v[3].x, v[3].y, T()));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int c = narrow_col<LANES, false>(l, i);
+            if (c < dim) p[c] = from_float<T>(i & 1 ? v[i / 2].y : v[i / 2].x);
+        }
+    }
+}
+
+template <int LANES>
+S3T_DEV float lanes_sum(float v) {
+#pragma unroll
+    for (int o = LANES / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+template <int LANES, bool VEC>
+S3T_DEV RowStats narrow_stats(const float2 (&v)[4], int layer, int dim, float inv_dim, float eps, int l) {
+    float mean = 0.f;
+    if (layer) {
+        const float2 t = __fadd2_rn(__fadd2_rn(v[0], v[1]), __fadd2_rn(v[2], v[3]));
+        mean = lanes_sum<LANES>(t.x + t.y) * inv_dim;
+    }
+    float2 q = both(0.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float2 d = __fadd2_rn(v[i], both(-mean));
+        if (narrow_col<LANES, VEC>(l, 2 * i) >= dim) d.x = 0.f;
+        if (narrow_col<LANES, VEC>(l, 2 * i + 1) >= dim) d.y = 0.f;
+        q = __ffma2_rn(d, d, q);
+    }
+    return {mean, rsqrtf(fmaf(lanes_sum<LANES>(q.x + q.y), inv_dim, eps))};
+}
+
+// A lane's elements of vector p: `otherwise` where there is none, 0 past dim.
+template <int LANES, bool VEC>
+S3T_DEV void narrow_vector(const float* p, float otherwise, int dim, int l, float2 (&v)[4]) {
+    if (p) {
+        NarrowRaw<float> raw;
+        narrow_load<LANES, VEC>(p, dim, l, true, raw);
+        narrow_widen(raw, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i].x = narrow_col<LANES, VEC>(l, 2 * i) < dim ? otherwise : 0.f;
+            v[i].y = narrow_col<LANES, VEC>(l, 2 * i + 1) < dim ? otherwise : 0.f;
+        }
+    }
+}
+
+// Rows of up to 8 LANES columns (heads, mostly): LANES lanes a row, so that no
+// lane idles, and the vectors in registers for all of a thread's rows.  82944
+// rows, fp16, LayerNorm twice: 128 columns 24 us (a warp a row, streamed: 49
+// us), 64 columns 14 us (48 us), 7 columns 6.3 us (58 us); 400000 x 128 86 us,
+// 4.8 TB/s, with the next row on its way (119 us without, bound by the loads'
+// latency at three CTAs an SM).
+template <typename T, typename R, int LANES, bool VEC>
+__global__ void __launch_bounds__(kNarrowThreads, 3) norm_narrow_kernel(const NormResidualArgs a) {
+    const int l = threadIdx.x % LANES, dim = a.dim;
+    const float inv_dim = 1.f / float(dim);
+    const uint32_t rows = uint32_t(a.rows), stride = gridDim.x * (kNarrowThreads / LANES);
+    const uint32_t in_warp = (threadIdx.x & 31) / LANES;
+    NarrowRaw<R> raw_x;
+    NarrowRaw<T> raw_y, raw_g;
+    auto load_x = [&](uint32_t row) {
+        narrow_load<LANES, VEC>(static_cast<const R*>(a.x) + int64_t(row) * a.x_stride, dim, l, row < rows, raw_x);
+    };
+    auto load_branch = [&](uint32_t row) {
+        const bool there = row < rows;
+        if (a.y) narrow_load<LANES, VEC>(static_cast<const T*>(a.y) + int64_t(row) * a.y_stride, dim, l, there, raw_y);
+        if (a.gate)
+            narrow_load<LANES, VEC>(static_cast<const T*>(a.gate) + int64_t(row / uint32_t(a.gate_rows)) * a.gate_stride, dim, l,
+                                    there, raw_g);
+    };
+    // The loop's bound is the warp's, for the shuffles.  The first row is asked
+    // for before the vectors: a call of a few rows is all latency.
+    uint32_t first = blockIdx.x * (kNarrowThreads / LANES) + (threadIdx.x & ~31u) / LANES;
+    load_branch(first + in_warp);
+    load_x(first + in_warp);
+    // As the streaming kernel's: the branch's scales folded in, 0 past dim.
+    float2 post_w[4], post_b[4], pre_w[4], pre_b[4];
+    {
+        float2 ch[4];
+        narrow_vector<LANES, VEC>(a.channel, 1.f, dim, l, ch);
+        narrow_vector<LANES, VEC>(a.post ? a.post_weight : nullptr, 1.f, dim, l, post_w);
+        narrow_vector<LANES, VEC>(a.post ? a.post_bias : nullptr, 0.f, dim, l, post_b);
+        narrow_vector<LANES, VEC>(a.pre_weight, 1.f, dim, l, pre_w);
+        narrow_vector<LANES, VEC>(a.pre_bias, 0.f, dim, l, pre_b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            ch[i] = __fmul2_rn(ch[i], both(a.branch_scale));
+            post_w[i] = __fmul2_rn(post_w[i], ch[i]);
+            post_b[i] = __fmul2_rn(post_b[i], ch[i]);
+        }
+    }
+    // The next row comes while this row's pre-norm runs.
+    while (first < rows) {
+        const uint32_t row = first + in_warp;
+        const bool there = row < rows;
+        first = rows - first > stride ? first + stride : rows;
+        float2 x[4], h[4];
+        if (a.y) {
+            narrow_widen(raw_y, h);
+            if (a.post) {
+                normalize(h, narrow_stats<LANES, VEC>(h, a.layer, dim, inv_dim, a.eps, l), post_w, post_b);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[i] = __fmul2_rn(h[i], post_w[i]);
+            }
+            if (a.gate) {
+                float2 g[4];
+                narrow_widen(raw_g, g);
+                apply_gate(h, g, a.gate_act);
+            }
+            narrow_widen(raw_x, x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = __ffma2_rn(both(a.resid_scale), x[i], h[i]);
+        } else {
+            narrow_widen(raw_x, x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = __fmul2_rn(both(a.resid_scale), x[i]);
+        }
+        if (first < rows) {
+            load_branch(first + in_warp);
+            load_x(first + in_warp);
+        }
+        if (a.x_out && there)
+            narrow_store<LANES, VEC>(static_cast<R*>(a.x_out) + int64_t(row) * a.x_out_stride, dim, l, x);
+        if (!a.u) continue;
+        normalize(x, narrow_stats<LANES, VEC>(x, a.layer, dim, inv_dim, a.eps, l), pre_w, pre_b);
+        if (!a.u_eight) {
+            if (there) narrow_store<LANES, VEC>(static_cast<T*>(a.u) + int64_t(row) * a.u_stride, dim, l, x);
+            continue;
+        }
+        // One scale group; columns past dim are zeros.
+        uint32_t peak = abs_bits(absmax3_nan(absmax3_nan(absmax3_nan(x[0].x, x[0].y, x[1].x), x[1].y, x[2].x),
+                                             absmax3_nan(x[2].y, x[3].x, x[3].y), 0.f));
+#pragma unroll
+        for (int o = LANES / 2; o; o >>= 1) peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+        const float top = __uint_as_float(max(peak, kAmaxFloorBits));
+        // Even lanes divide for the scale, odd ones for its inverse.
+        const float quotient = __fdiv_rn(l & 1 ? kE4M3Max : top, l & 1 ? top : kE4M3Max);
+        const float2 inv = both(__shfl_sync(0xffffffffu, quotient, 1, LANES));
+        float2 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __fmul2_rn(x[i], inv);
+        const uint32_t lo = pack_e4m3x4(v[0].x, v[0].y, v[1].x, v[1].y), hi = pack_e4m3x4(v[2].x, v[2].y, v[3].x, v[3].y);
+        if (!there) continue;
+        uint8_t* q = static_cast<uint8_t*>(a.u) + int64_t(row) * a.u_stride;
+        if constexpr (VEC) {
+            if (l * 8 < dim) *reinterpret_cast<uint2*>(q + l * 8) = make_uint2(lo, hi);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int c = narrow_col<LANES, false>(l, i);
+                if (c < dim) q[c] = uint8_t((i < 4 ? lo : hi) >> (8 * (i & 3)));
+            }
+        }
+        if (l == 0) a.u_scale[row] = quotient;
+    }
+}
+
+template <typename T, typename R, int LANES>
+cudaError_t launch_narrow(const NormResidualArgs& a, int num_sms, cudaStream_t stream) {
+    const int64_t ctas = (a.rows * LANES + kNarrowThreads - 1) / kNarrowThreads;
+    const uint32_t grid = uint32_t(ctas < 3 * num_sms ? ctas : 3 * num_sms);
+    if (a.vec) norm_narrow_kernel<T, R, LANES, true><<<grid, kNarrowThreads, 0, stream>>>(a);
+    else norm_narrow_kernel<T, R, LANES, false><<<grid, kNarrowThreads, 0, stream>>>(a);
+    return cudaGetLastError();
+}
+
 template <typename T, typename R, int CPW, bool VEC>
 cudaError_t launch_few(const NormResidualArgs& a, cudaStream_t stream) {
     const int warps = (a.dim + CPW * kChunk - 1) / (CPW * kChunk);
@@ -556,6 +779,9 @@ bool launch_stream(const NormResidualArgs& a, int num_sms, cudaStream_t stream) 
 
 template <typename T, typename R>
 cudaError_t launch_types(const NormResidualArgs& a, int num_sms, cudaStream_t stream) {
+    if (a.dim <= 32) return launch_narrow<T, R, 4>(a, num_sms, stream);
+    if (a.dim <= 64) return launch_narrow<T, R, 8>(a, num_sms, stream);
+    if (a.dim <= 128) return launch_narrow<T, R, 16>(a, num_sms, stream);
     const bool streamed = a.dim <= kChunk       ? launch_stream<T, R, 1>(a, num_sms, stream)
                           : a.dim <= 2 * kChunk ? launch_stream<T, R, 2>(a, num_sms, stream)
                                                 : launch_stream<T, R, 4>(a, num_sms, stream);

@@ -433,6 +433,28 @@ def test_norm_streams_of_rows(torch, kind, resid, rows, dim, pad):
     run_norm(torch, 12, rows, dim, kind, resid, branch=False, layer=True, weights=False, pad=pad, write_x=False)
 
 
+@pytest.mark.parametrize("kind, resid", TYPE_PAIRS)
+@pytest.mark.parametrize("rows, dim, pad", [(1, 128, 0), (6, 127, 0), (1, 1, 0), (131, 64, 0), (67, 65, 3), (300, 32, 8), (129, 33, 1),
+                                            (30001, 31, 0), (40007, 128, 0), (30003, 80, 1), (60005, 16, 0)])
+def test_norm_narrow_rows(torch, kind, resid, rows, dim, pad):
+    """Several rows a warp: whole and ragged warps, more rows than the grid takes at once."""
+    run_norm(torch, 13, rows, dim, kind, resid, layer=True, gate="sigmoid", gate_rows=5, eight=True, pad=pad)
+    run_norm(torch, 14, rows, dim, kind, resid, gate="tanh", gate_rows=1000, pad=pad, in_place=True, branch_scale=0.25)
+    run_norm(torch, 15, rows, dim, kind, resid, branch=False, weights=False, pad=pad, write_x=False)
+    run_norm(torch, 16, rows, dim, kind, resid, post=False, channel=False, layer=True, write_u=False, pad=pad)
+
+
+def test_norm_narrow_nonfinite_rows_stay_apart(torch):
+    rows, dim = 70, 64
+    x = torch.randn(rows, dim, device="cuda")
+    x[9, 3], x[34, 4] = float("nan"), -float("inf")
+    u = Eight(torch, rows, dim)
+    s3t.norm_residual(0, s3t.NormArgs(rows=rows, dim=dim, type=0, resid_type=0, u_type=s3t.TYPE_E4M3, flags=s3t.NORM_LAYER,
+                                      eps=1e-5, resid_scale=1.0, x=x.data_ptr(), x_stride=dim, u=u.matrix))
+    bad = torch.isnan(u.values(torch))
+    assert bad[9].all() and bad[34].all() and int(bad.any(1).sum()) == 2 and u.untouched()
+
+
 def test_norm_parts_that_are_left_out(torch):
     for dim in (256, 515):
         run_norm(torch, 1, 9, dim, "f16", "f32", branch=False)                                  # a pre-norm alone
