@@ -25,7 +25,8 @@
 // latency), one chunk a warp with the next row in registers 269 us (four times
 // the reductions).
 // Few rows: one chunk a warp up to 4096 columns, everything asked for at once,
-// for the latency of one row.
+// for the latency of one row; up to 32 warps of one or two chunks above (2 x
+// 16384: 6.7 us, with 16 warps of four chunks 7.8 us; 4 x 6791 7.6 and 11.6 us).
 //
 // Up to 128 columns: several rows a warp (norm_narrow_kernel).
 //
@@ -43,7 +44,7 @@ namespace s3t {
 namespace {
 
 constexpr int kChunk = 2 * kScaleBlock;
-constexpr int kMaxWarps = 16;          // of a team: 16 x 4 chunks hold kNormMaxDim columns
+constexpr int kMaxWarps = 16;          // of a team with four chunks (kNormMaxDim columns) or one with its vectors a warp
 constexpr int kSlots = 1;              // rows ahead of a warp (STREAM)
 constexpr int kStreamWarps = 16;
 constexpr int kNarrowThreads = 256;
@@ -283,10 +284,10 @@ S3T_DEV void store_eight(const NormResidualArgs& a, uint32_t row, int c0, int la
 }
 
 // Few rows: a team of blockDim.x / 32 warps takes one row, blockDim.y teams a CTA.
-template <typename T, typename R, int CPW, bool VEC>
-__global__ void __launch_bounds__(32 * kMaxWarps) norm_rows_kernel(const NormResidualArgs a) {
-    __shared__ float2 exchange[4][2][kMaxWarps];
-    constexpr bool KEEP = CPW == 1;      // the vectors fit registers: asked for with the row
+// KEEP: the vectors fit registers and are asked for with the row.
+template <typename T, typename R, int CPW, bool KEEP, bool VEC>
+__global__ void __launch_bounds__(32 * (KEEP ? kMaxWarps : 2 * kMaxWarps)) norm_rows_kernel(const NormResidualArgs a) {
+    __shared__ float2 exchange[4][2][2 * kMaxWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, team = threadIdx.y;
     const int dim = a.dim, last = dim - (warps - 1) * CPW * kChunk;
     const Split sp{lane, warp, warps, team, last, 1.f / float(dim), 1.f / float(last)};
@@ -353,15 +354,22 @@ __global__ void __launch_bounds__(32 * kMaxWarps) norm_rows_kernel(const NormRes
     if (a.u_eight) store_eight<CPW, VEC>(a, row, c0, lane, x);
 }
 
-// Shared memory of a streaming CTA: the vectors, each a row of floats padded
-// to its team's columns; then per warp kSlots rows of its columns of x, y and
-// gate; then the barriers.
+// Shared memory of a streaming CTA: the vectors that the call has, each a row of
+// floats padded to its team's columns; then per warp kSlots rows of its columns
+// of x, y and gate, as far as there are; then the barriers.
 template <typename T, typename R, int CPW>
 struct StreamRow {
     static constexpr uint32_t COLS = CPW * kChunk;
     static constexpr uint32_t X = COLS * sizeof(R) + 16, Y = COLS * sizeof(T) + 16;   // and what lies around them
-    static constexpr uint32_t BYTES = X + 2 * Y;
 };
+// Vector k: post weight and post bias with the branch's scales, pre weight, pre bias.
+__host__ __device__ inline bool has_vector(const NormResidualArgs& a, int k) {
+    return k == 0 ? a.y != nullptr : k == 1 ? a.post && a.post_bias : k == 2 ? a.u != nullptr : a.u && a.pre_bias;
+}
+template <typename Row>
+__host__ __device__ uint32_t row_bytes(const NormResidualArgs& a) {
+    return Row::X + (a.y ? Row::Y : 0) + (a.gate ? Row::Y : 0);
+}
 
 // The 16-byte units that hold `bytes` bytes from p on.
 S3T_DEV uint32_t units_around(const void* p, uint32_t bytes) {
@@ -385,22 +393,25 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
     const int dim = a.dim, last = dim - (warps - 1) * int(Row::COLS), padded = warps * int(Row::COLS);
     const Split sp{lane, warp, warps, team, last, 1.f / float(dim), 1.f / float(last)};
     const int c0 = warp * int(Row::COLS), cols = warp + 1 == warps ? last : int(Row::COLS);
-    float* vec = reinterpret_cast<float*>(words);
-    {
-        // Weight and bias of the branch with its scales folded in (the bias only
-        // with a post-norm), then those of the pre-norm; 0 past dim.
-        for (int c = thread; c < padded; c += threads) {
-            const bool in = c < dim;
+    float* const vec0 = reinterpret_cast<float*>(words);
+    float* const vec1 = vec0 + (has_vector(a, 0) ? padded : 0);
+    float* const vec2 = vec1 + (has_vector(a, 1) ? padded : 0);
+    float* const vec3 = vec2 + (has_vector(a, 2) ? padded : 0);
+    uint8_t* const buffers = reinterpret_cast<uint8_t*>(vec3 + (has_vector(a, 3) ? padded : 0));
+    for (int c = thread; c < padded; c += threads) {   // 0 past dim
+        const bool in = c < dim;
+        if (has_vector(a, 0)) {
             const float s = in ? a.branch_scale * (a.channel ? a.channel[c] : 1.f) : 0.f;
-            vec[c] = a.post && a.post_weight && in ? a.post_weight[c] * s : s;
-            vec[padded + c] = a.post && a.post_bias && in ? a.post_bias[c] * s : 0.f;
-            vec[2 * padded + c] = in ? (a.pre_weight ? a.pre_weight[c] : 1.f) : 0.f;
-            vec[3 * padded + c] = a.pre_bias && in ? a.pre_bias[c] : 0.f;
+            vec0[c] = a.post && a.post_weight && in ? a.post_weight[c] * s : s;
+            if (has_vector(a, 1)) vec1[c] = in ? a.post_bias[c] * s : 0.f;
         }
+        if (has_vector(a, 2)) vec2[c] = in ? (a.pre_weight ? a.pre_weight[c] : 1.f) : 0.f;
+        if (has_vector(a, 3)) vec3[c] = in ? a.pre_bias[c] : 0.f;
     }
+    const uint32_t bytes = row_bytes<Row>(a);
     // VEC: columns past dim are never copied, they stay zeros.
-    uint8_t* mine = reinterpret_cast<uint8_t*>(vec + kStreamVectors * padded) + (team * warps + warp) * kSlots * Row::BYTES;
-    for (uint32_t i = lane; i < kSlots * Row::BYTES / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
+    uint8_t* mine = buffers + (team * warps + warp) * kSlots * bytes;
+    for (uint32_t i = lane; i < kSlots * bytes / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
     uint64_t* bar = arrived[team * warps + warp];
     if (lane == 0) {
         for (int i = 0; i < kSlots; ++i) mbar_init(bar + i, 1);
@@ -419,7 +430,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
     uint32_t ahead = row;
     auto fetch = [&](int slot) {       // one lane
         if (ahead >= rows) return;
-        uint8_t* to = mine + slot * Row::BYTES;
+        uint8_t* to = mine + slot * bytes;
         const uint32_t xb = uint32_t(cols) * sizeof(R), tb = uint32_t(cols) * sizeof(T);
         const T* gp = static_cast<const T*>(a.gate);
         if (a.gate) gp += int64_t(ahead / uint32_t(a.gate_rows)) * a.gate_stride + c0;
@@ -452,9 +463,17 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
             lost = true;
             mbar_wait(bar + slot, (it / kSlots) & 1, a.status, kErrTimeoutDrain, nullptr);
         }
-        const uint8_t* from = mine + slot * Row::BYTES;
+        const uint8_t* from = mine + slot * bytes;
         float2 x[CPW][4], h[CPW][4];
-        auto vector = [&](int k, int j, float2(&v)[4]) { load_chunk<VEC>(vec + k * padded + c0 + j * kChunk, 0, kChunk, lane, v); };
+        auto vector = [&](const float* p, int j, float2(&v)[4]) { load_chunk<VEC>(p + c0 + j * kChunk, 0, kChunk, lane, v); };
+        auto bias = [&](const float* p, bool there, int j, float2(&v)[4]) {
+            if (there) {
+                vector(p, j, v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = both(0.f);
+            }
+        };
         // Chunk j of a row whose units lie at p and which begins where `at` says.
         auto chunk = [&](const uint8_t* p, auto* at, int j, float2(&v)[4]) {
             using E = typename std::remove_const<typename std::remove_pointer<decltype(at)>::type>::type;
@@ -470,15 +489,15 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
 #pragma unroll
                 for (int j = 0; j < CPW; ++j) {
                     float2 w[4], b[4];
-                    vector(0, j, w);
-                    vector(1, j, b);
+                    vector(vec0, j, w);
+                    bias(vec1, has_vector(a, 1), j, b);
                     normalize(h[j], st, w, b);
                 }
             } else {
 #pragma unroll
                 for (int j = 0; j < CPW; ++j) {
                     float2 w[4];
-                    vector(0, j, w);
+                    vector(vec0, j, w);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) h[j][i] = __fmul2_rn(h[j][i], w[i]);
                 }
@@ -518,8 +537,8 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
 #pragma unroll
             for (int j = 0; j < CPW; ++j) {
                 float2 w[4], b[4];
-                vector(2, j, w);
-                vector(3, j, b);
+                vector(vec2, j, w);
+                bias(vec3, has_vector(a, 3), j, b);
                 normalize(x[j], st, w, b);
                 if (!a.u_eight)
                     store_chunk<VEC>(static_cast<T*>(a.u) + int64_t(row) * a.u_stride, c0 + j * kChunk, dim, lane, x[j]);
@@ -751,12 +770,14 @@ cudaError_t launch_narrow(const NormResidualArgs& a, int num_sms, cudaStream_t s
     return cudaGetLastError();
 }
 
-template <typename T, typename R, int CPW, bool VEC>
+template <typename T, typename R, int CPW, bool KEEP>
 cudaError_t launch_few(const NormResidualArgs& a, cudaStream_t stream) {
     const int warps = (a.dim + CPW * kChunk - 1) / (CPW * kChunk);
     const int teams = warps == 1 ? 4 : 1;
     const int64_t ctas = (a.rows + teams - 1) / teams;
-    norm_rows_kernel<T, R, CPW, VEC><<<uint32_t(ctas), dim3(32 * warps, teams), 0, stream>>>(a);
+    const dim3 block(32 * warps, teams);
+    if (a.vec) norm_rows_kernel<T, R, CPW, KEEP, true><<<uint32_t(ctas), block, 0, stream>>>(a);
+    else norm_rows_kernel<T, R, CPW, KEEP, false><<<uint32_t(ctas), block, 0, stream>>>(a);
     return cudaGetLastError();
 }
 
@@ -765,13 +786,21 @@ template <typename T, typename R, int CPW>
 bool launch_stream(const NormResidualArgs& a, int num_sms, cudaStream_t stream) {
     using Row = StreamRow<T, R, CPW>;
     const int warps = (a.dim + int(Row::COLS) - 1) / int(Row::COLS);
-    const int vector_bytes = kStreamVectors * warps * int(Row::COLS) * 4;
-    int teams = vector_bytes < kStreamBytes ? (kStreamBytes - vector_bytes) / (warps * kSlots * int(Row::BYTES)) : 0;
+    int vectors = 0;
+    for (int k = 0; k < kStreamVectors; ++k) vectors += has_vector(a, k);
+    const int vector_bytes = vectors * warps * int(Row::COLS) * 4, team_bytes = warps * kSlots * int(row_bytes<Row>(a));
+    int teams = vector_bytes < kStreamBytes ? (kStreamBytes - vector_bytes) / team_bytes : 0;
     if (teams > kStreamWarps / warps) teams = kStreamWarps / warps;
     // Two rows a team and more: the rows ahead pay for the set-up.
     if (teams == 0 || a.rows < int64_t(2) * num_sms * teams) return false;
+    // Fewer than ten warps an SM hide too little, unless the call has more vectors
+    // than the other kernel had better read again for every row (streamed / not:
+    // 719 x 7070 fp32, 7 warps, 77 / 35 us; 2290 x 9024 fp16, 9 warps, 91 / 85
+    // us; 2290 x 8192 fp16 with four vectors, 8 warps, 85 / 114 us; 5000 x 5120
+    // bf16, 15 warps, 54 / 69 us; 5000 x 16384 fp16, 16 warps, 169 / 238 us).
+    if (teams * warps < 10 && vectors <= 2) return false;
     const dim3 block(32 * warps, teams);
-    const uint32_t smem = uint32_t(vector_bytes) + uint32_t(teams * warps) * kSlots * Row::BYTES;
+    const uint32_t smem = uint32_t(vector_bytes + teams * team_bytes);
     if (a.vec) norm_stream_kernel<T, R, CPW, true><<<num_sms, block, smem, stream>>>(a);
     else norm_stream_kernel<T, R, CPW, false><<<num_sms, block, smem, stream>>>(a);
     return true;
@@ -786,8 +815,9 @@ cudaError_t launch_types(const NormResidualArgs& a, int num_sms, cudaStream_t st
                           : a.dim <= 2 * kChunk ? launch_stream<T, R, 2>(a, num_sms, stream)
                                                 : launch_stream<T, R, 4>(a, num_sms, stream);
     if (streamed) return cudaGetLastError();
-    if (a.dim <= kMaxWarps * kChunk) return a.vec ? launch_few<T, R, 1, true>(a, stream) : launch_few<T, R, 1, false>(a, stream);
-    return a.vec ? launch_few<T, R, 4, true>(a, stream) : launch_few<T, R, 4, false>(a, stream);
+    if (a.dim <= kMaxWarps * kChunk) return launch_few<T, R, 1, true>(a, stream);
+    if (a.dim <= 2 * kMaxWarps * kChunk) return launch_few<T, R, 1, false>(a, stream);
+    return launch_few<T, R, 2, false>(a, stream);
 }
 
 template <typename T, typename R, int CPW>

@@ -455,6 +455,17 @@ def test_norm_narrow_nonfinite_rows_stay_apart(torch):
     assert bad[9].all() and bad[34].all() and int(bad.any(1).sum()) == 2 and u.untouched()
 
 
+@pytest.mark.parametrize("kind, resid", TYPE_PAIRS)
+@pytest.mark.parametrize("rows, dim, pad", [(5, 4097, 0), (9, 8192, 0), (3, 8193, 3), (620, 5120, 0), (310, 7001, 1), (300, 8200, 0),
+                                            (301, 9024, 0), (299, 12289, 0), (330, 16384, 0)])
+def test_norm_wide_rows(torch, kind, resid, rows, dim, pad):
+    """Rows of 5 to 16 streaming warps, and those that one CTA a row takes."""
+    run_norm(torch, 17, rows, dim, kind, resid, layer=True, gate="sigmoid", gate_rows=3, eight=True, pad=pad)
+    run_norm(torch, 18, rows, dim, kind, resid, weights=False, pad=pad, in_place=True)
+    run_norm(torch, 19, rows, dim, kind, resid, branch=False, pad=pad, write_x=False)
+    run_norm(torch, 20, rows, dim, kind, resid, post=False, weights=False, gate="plain", write_u=False, pad=pad)
+
+
 def test_norm_parts_that_are_left_out(torch):
     for dim in (256, 515):
         run_norm(torch, 1, 9, dim, "f16", "f32", branch=False)                                  # a pre-norm alone
