@@ -28,7 +28,7 @@
 // for the latency of one row; up to 32 warps of one or two chunks above (2 x
 // 16384: 6.7 us, with 16 warps of four chunks 7.8 us; 4 x 6791 7.6 and 11.6 us).
 //
-// Up to 128 columns: several rows a warp (norm_narrow_kernel).
+// Up to 256 columns: eight a lane, several rows a warp (norm_narrow_kernel).
 //
 // A LayerNorm warp reduces its own mean and centred square sum and the warps'
 // are merged about the row's mean (Chan, Golub and LeVeque, 1979), so there is
@@ -550,12 +550,15 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) norm_stream_kernel(const
     }
 }
 
-// ------------------------------------------------------- rows up to 128 ---
+// ------------------------------------------------------- rows up to 256 ---
 
-// Columns of element i of a lane's eight, LANES lanes a row.
+// Columns of element i of a lane's eight, LANES lanes a row; 16 lanes hold a
+// group of 128.
 template <int LANES, bool VEC>
 S3T_DEV int narrow_col(int l, int i) {
-    return VEC ? l * 8 + i : l + LANES * i;
+    if constexpr (VEC) return l * 8 + i;
+    else if constexpr (LANES <= 16) return l + LANES * i;
+    else return (l / 16) * kScaleBlock + l % 16 + 16 * i;
 }
 
 // A lane's elements as they lie in memory: widened where they are used, since
@@ -733,15 +736,16 @@ __global__ void __launch_bounds__(kNarrowThreads, 3) norm_narrow_kernel(const No
             if (there) narrow_store<LANES, VEC>(static_cast<T*>(a.u) + int64_t(row) * a.u_stride, dim, l, x);
             continue;
         }
-        // One scale group; columns past dim are zeros.
+        // Columns past dim are zeros.
+        constexpr int GROUP = LANES < 16 ? LANES : 16;       // lanes of a scale group
         uint32_t peak = abs_bits(absmax3_nan(absmax3_nan(absmax3_nan(x[0].x, x[0].y, x[1].x), x[1].y, x[2].x),
                                              absmax3_nan(x[2].y, x[3].x, x[3].y), 0.f));
 #pragma unroll
-        for (int o = LANES / 2; o; o >>= 1) peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+        for (int o = GROUP / 2; o; o >>= 1) peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, o));
         const float top = __uint_as_float(max(peak, kAmaxFloorBits));
         // Even lanes divide for the scale, odd ones for its inverse.
         const float quotient = __fdiv_rn(l & 1 ? kE4M3Max : top, l & 1 ? top : kE4M3Max);
-        const float2 inv = both(__shfl_sync(0xffffffffu, quotient, 1, LANES));
+        const float2 inv = both(__shfl_sync(0xffffffffu, quotient, 1, GROUP));
         float2 v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = __fmul2_rn(x[i], inv);
@@ -757,7 +761,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 3) norm_narrow_kernel(const No
                 if (c < dim) q[c] = uint8_t((i < 4 ? lo : hi) >> (8 * (i & 3)));
             }
         }
-        if (l == 0) a.u_scale[row] = quotient;
+        if (l % GROUP == 0 && l * 8 < dim) a.u_scale[int64_t(l / 16) * a.u_scale_stride + row] = quotient;
     }
 }
 
@@ -811,7 +815,11 @@ cudaError_t launch_types(const NormResidualArgs& a, int num_sms, cudaStream_t st
     if (a.dim <= 32) return launch_narrow<T, R, 4>(a, num_sms, stream);
     if (a.dim <= 64) return launch_narrow<T, R, 8>(a, num_sms, stream);
     if (a.dim <= 128) return launch_narrow<T, R, 16>(a, num_sms, stream);
-    const bool streamed = a.dim <= kChunk       ? launch_stream<T, R, 1>(a, num_sms, stream)
+    // A CTA of eight rows on every SM, a warp each: 82944 x 256 fp16 45 us, streamed
+    // 55 us; with fewer rows one warp a row of the other kernel is as good (1000 x
+    // 256 2.8 and 2.7 us).
+    if (a.dim <= kChunk && a.rows >= 8 * num_sms) return launch_narrow<T, R, 32>(a, num_sms, stream);
+    const bool streamed = a.dim <= kChunk       ? false
                           : a.dim <= 2 * kChunk ? launch_stream<T, R, 2>(a, num_sms, stream)
                                                 : launch_stream<T, R, 4>(a, num_sms, stream);
     if (streamed) return cudaGetLastError();
@@ -831,7 +839,6 @@ cudaError_t prepare_stream() {
 template <typename T, typename R>
 cudaError_t prepare_types() {
     cudaError_t e;
-    if ((e = prepare_stream<T, R, 1>()) != cudaSuccess) return e;
     if ((e = prepare_stream<T, R, 2>()) != cudaSuccess) return e;
     return prepare_stream<T, R, 4>();
 }

@@ -435,7 +435,8 @@ def test_norm_streams_of_rows(torch, kind, resid, rows, dim, pad):
 
 @pytest.mark.parametrize("kind, resid", TYPE_PAIRS)
 @pytest.mark.parametrize("rows, dim, pad", [(1, 128, 0), (6, 127, 0), (1, 1, 0), (131, 64, 0), (67, 65, 3), (300, 32, 8), (129, 33, 1),
-                                            (30001, 31, 0), (40007, 128, 0), (30003, 80, 1), (60005, 16, 0)])
+                                            (30001, 31, 0), (40007, 128, 0), (30003, 80, 1), (60005, 16, 0),
+                                            (1184, 129, 0), (9001, 256, 0), (5003, 200, 8), (7001, 255, 1)])
 def test_norm_narrow_rows(torch, kind, resid, rows, dim, pad):
     """Several rows a warp: whole and ragged warps, more rows than the grid takes at once."""
     run_norm(torch, 13, rows, dim, kind, resid, layer=True, gate="sigmoid", gate_rows=5, eight=True, pad=pad)
