@@ -44,7 +44,7 @@ namespace s3t {
 namespace {
 
 constexpr int kChunk = 2 * kScaleBlock;
-constexpr int kMaxWarps = 16;          // of a team with four chunks (kNormMaxDim columns) or one with its vectors a warp
+constexpr int kMaxWarps = 16;          // of a row whose vectors stay in registers; twice as many where they do not
 constexpr int kSlots = 1;              // rows ahead of a warp (STREAM)
 constexpr int kStreamWarps = 16;
 constexpr int kNarrowThreads = 256;
