@@ -295,10 +295,12 @@ int s3t_quantize_fp8(int device, int type, const void *x_dev, int64_t rows, int6
 /* y[M][N] = act(x[M][K] * w[N][K]^T + bias) of an e4m3 activation x (row
  * blocks of 1) and an e4m3 weight w (row blocks of 128): the products of a
  * group of 128 columns are summed in fp32 and scaled by both scales, the
- * groups are summed in fp32.  bias: [N] fp32 or NULL.  act: 0 none, 1 GELU-erf
- * (as s3t_gemm_f16).  y_type: F32, F16, BF16, or E4M3, which quantizes the
- * result as s3t_quantize_fp8 does with block_rows 1 (y->scale for [ceil(N /
- * 128)][scale_stride >= M]), ready to be the next product's x.  Any M, N >= 0
+ * groups are summed in fp32.  bias: [N] fp32 or NULL.  act: 0 none, 1 GELU-erf,
+ * computed in fp32 to within 1.9e-7 |x| and, for x >= -6, 2.4e-4 of GELU(x)
+ * itself (below, where |GELU| < 6e-9, it falls to 0 sooner than GELU).  y_type:
+ * F32, F16, BF16, or E4M3, which holds what s3t_quantize_fp8 with block_rows 1
+ * makes of the F32 result (y->scale for [ceil(N / 128)][scale_stride >= M]),
+ * ready to be the next product's x.  Any M, N >= 0
  * and K >= 1, up to 2^30 each.  The result does not depend on what else runs.  A wait that runs
  * out inside the kernel is reported by s3t_device_status. */
 int s3t_gemm_fp8(int device, const s3t_matrix *x, const s3t_matrix *w, const float *bias_dev, int M, int N, int K,

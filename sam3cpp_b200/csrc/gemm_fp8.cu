@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(192)
             if (args.gelu) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float2 t = gelu_erf_poly2<OUT != kE4M3>(make_float2(v[2 * i], v[2 * i + 1]));
+                    const float2 t = gelu_erf_poly2(make_float2(v[2 * i], v[2 * i + 1]));
                     v[2 * i] = t.x;
                     v[2 * i + 1] = t.y;
                 }
@@ -724,7 +724,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
             if (n0 >= args.N || row0 >= args.M) continue;   // warp-uniform: nothing of y here
             if (args.gelu) {
 #pragma unroll
-                for (int i = 0; i < Cfg::WARP_COLS / 2; ++i) sum[i] = gelu_erf_poly2<OUT != kE4M3>(sum[i]);
+                for (int i = 0; i < Cfg::WARP_COLS / 2; ++i) sum[i] = gelu_erf_poly2(sum[i]);
             }
             // Each lane writes 128 bytes of its row at a time to a swizzled stage,
             // and one TMA store per warp takes the 32 rows while the next tile is

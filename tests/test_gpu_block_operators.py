@@ -245,6 +245,37 @@ def test_product_gelu_by_its_argument(torch, m, out):
     assert (err <= (e + (want.abs() + e) * half + tiny)[3:]).all(), float((err - e[3:]).max())
 
 
+@pytest.mark.parametrize("m", [3, 100, 2600])
+@pytest.mark.parametrize("n", [129, 256, 300])
+@pytest.mark.parametrize("low, high", [(-5.0, -2.0), (-6.0, -4.5), (-3.0, 3.0), (-1e-3, 1e-3), (-40.0, -9.0)])
+def test_product_gelu_block_scales(torch, m, n, low, high):
+    """Zero products: a block's 8 bits are GELU(bias) as the same call answers it in fp32, quantized, and its scale is
+    the block's largest GELU / 448, also where all of a block lies in GELU's tail (or the last block is one column).
+    GELU is within 2.3e-4 of its value down to -6, by at most 2.3e-4 + 2^-22 + eight roundings of partial sums no
+    larger than 1 + |log2 Q| of the exponent, each worth ln 2 of it."""
+    x, w = Eight(torch, m, 130), Eight(torch, n, 130, 128)
+    for t in (x, w):
+        t.q[:] = 0
+        t.scale[:] = 1
+    b = torch.linspace(low, high, n, device="cuda")
+    y8, y = call_product(torch, x, w, b, True, "e4m3"), call_product(torch, x, w, b, True, "f32")[:m]
+    codes, scales = quantized(torch, y, 1)
+    assert torch.equal(y8.scales(), scales)
+    assert torch.equal(y8.codes(torch).float(), codes.float())
+    v = b.double()
+    q = torch.special.erfc(v.abs() * math.sqrt(0.5)) / 2
+    want = 0.5 * v * torch.special.erfc(-v * math.sqrt(0.5))
+    if low < -6:                    # tiny, and never above what is left at -9
+        assert (y <= 0).all() and (y.abs() <= 1.1e-18).all()
+        return
+    rel = 2.3e-4 + 2.0 ** -22 + 8 * U * math.log(2) * (1 + q.log2().abs()) + 3 * U
+    assert ((y.double() - want).abs() <= want.abs() * rel).all()
+    top = torch.zeros(up(n, 128), device="cuda", dtype=torch.float64)
+    top[:n] = want.abs()
+    top = top.view(-1, 128).amax(1) / 448
+    assert ((y8.scales().double() / top[:, None] - 1).abs() <= float(rel.max()) + 4 * U).all()
+
+
 LARGE = [(2048, 1024, 1024), (2500, 4736, 1024), (5184, 1000, 4736), (4097, 129, 100), (20000, 512, 100), (3000, 257, 4000),
          (30011, 11, 500), (9000, 1, 1)]
 
