@@ -316,6 +316,11 @@ __global__ void __launch_bounds__(192)
             T* row = static_cast<T*>(args.y) + int64_t(m) * args.y_stride;
             const bool whole = args.vec && n + 4 <= args.N;
             if constexpr (OUT == kE4M3) {
+                // Columns past N take no part in the block: their products are 0,
+                // and NaN under an infinite scale.
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (n + i >= args.N) v[i] = 0.f;
                 uint32_t a = max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
                 a = __reduce_max_sync(0xffffffffu, a);
                 const BlockScale s = block_scale(a);
@@ -741,7 +746,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg8::THREADS, 1
                 float a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < Cfg::WARP_COLS / 2; ++i) a[i & 3] = absmax3_nan(a[i & 3], sum[i].x, sum[i].y);
-                bs = block_scale(__float_as_uint(absmax3_nan(absmax3_nan(a[0], a[1], a[2]), a[3], a[3])) & 0x7fffffffu);
+                float top = absmax3_nan(absmax3_nan(a[0], a[1], a[2]), a[3], a[3]);
+                // As in the tile kernel, columns past N take no part.  Looked at again only
+                // where they can matter, and by steps that stay in this branch:
+                // masks that the compiler may compute ahead spill (fc1 48.9 -> 62.8 us).
+                const int left = args.N - n0;
+                if (left < Cfg::WARP_COLS && top != top) {
+                    top = 0.f;
+#pragma unroll
+                    for (int i = 0; i < Cfg::WARP_COLS / 2; ++i) {
+                        absmax_nan_if(top, sum[i].x, 2 * i, left);
+                        absmax_nan_if(top, sum[i].y, 2 * i + 1, left);
+                    }
+                }
+                bs = block_scale(abs_bits(top));
                 if (row0 + lane < args.M) args.ys[int64_t(n0 / kScaleBlock) * args.ys_stride + row0 + lane] = bs.scale;
             }
 #pragma unroll

@@ -513,6 +513,13 @@ S3T_DEV float absmax3_nan(float a, float b, float c) {
     return d;
 }
 
+// top = the largest magnitude of top and v where i < n (NaN if one is NaN),
+// never moved or computed ahead.
+S3T_DEV void absmax_nan_if(float& top, float v, int i, int n) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.s32 p, %2, %3;\n\t@p max.NaN.abs.f32 %0, %0, %1, %1;\n\t}"
+                 : "+f"(top) : "f"(v), "r"(i), "r"(n));
+}
+
 S3T_DEV void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 S3T_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 

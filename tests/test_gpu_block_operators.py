@@ -308,6 +308,45 @@ def test_product_nonfinite_rows_stay_apart(torch, m):
     assert torch.equal(torch.isnan(y), bad)
 
 
+@pytest.mark.parametrize("m", [4, 150, 2600])
+@pytest.mark.parametrize("out", ["f32", "e4m3"])
+@pytest.mark.parametrize("gelu", [False, True])
+def test_product_infinite_scales(torch, m, out, gelu):
+    """What a quantized block with an infinity leaves as its scale: its row (or its block of columns) becomes infinite,
+    which 8 bits hold as an infinite scale, also where the block ends before 128 columns; all else stays as it was."""
+    g = torch.Generator("cuda").manual_seed(3)
+    n, k = 200, 300
+    x, w = random_eight(torch, g, m, k, 1), random_eight(torch, g, n, k, 128)
+    x.q &= 0x7F                     # no sum of a group is 0: even columns are positive, odd ones negative
+    w.q &= 0x7F
+    w.q[1:n:2] |= 0x80
+    inf = float("inf")
+    ends = torch.tensor([inf, 0.0 if gelu else -inf], device="cuda").repeat(n // 2)
+
+    def call():
+        y = call_product(torch, x, w, None, gelu, out)
+        return (y.codes(torch).float(), y.scales().t()) if out == "e4m3" else (y[:m].clone(), None)
+
+    before, before_scale = call()
+    kept = float(x.scale[1, 3])
+    x.scale[1, 3] = inf
+    y, scale = call()
+    others = torch.arange(m, device="cuda") != 3
+    assert torch.equal(y[others], before[others])
+    if out == "e4m3":
+        assert (scale[3] == inf).all() and torch.equal(scale[others], before_scale[others])
+    else:
+        assert torch.equal(y[3], ends)
+    x.scale[1, 3] = kept
+    w.scale[2, 1] = inf
+    y, scale = call()
+    assert torch.equal(y[:, :128], before[:, :128])
+    if out == "e4m3":
+        assert torch.equal(scale[:, 0], before_scale[:, 0]) and (scale[:, 1] == inf).all()
+    else:
+        assert torch.equal(y[:, 128:], ends[128:].expand(m, -1))
+
+
 @pytest.mark.parametrize("m, n, k", [(1, 4736, 1024), (100, 1024, 4736), (2600, 1024, 512)])
 def test_product_repeats_on_streams_and_in_graphs(torch, m, n, k):
     g = torch.Generator("cuda").manual_seed(11)
