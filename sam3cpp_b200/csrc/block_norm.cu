@@ -769,9 +769,8 @@ template <typename T, typename R, int LANES>
 cudaError_t launch_narrow(const NormResidualArgs& a, int num_sms, cudaStream_t stream) {
     const int64_t ctas = (a.rows * LANES + kNarrowThreads - 1) / kNarrowThreads;
     const uint32_t grid = uint32_t(ctas < 3 * num_sms ? ctas : 3 * num_sms);
-    if (a.vec) norm_narrow_kernel<T, R, LANES, true><<<grid, kNarrowThreads, 0, stream>>>(a);
-    else norm_narrow_kernel<T, R, LANES, false><<<grid, kNarrowThreads, 0, stream>>>(a);
-    return cudaGetLastError();
+    if (a.vec) return launch_on(norm_narrow_kernel<T, R, LANES, true>, grid, kNarrowThreads, 0, stream, a);
+    return launch_on(norm_narrow_kernel<T, R, LANES, false>, grid, kNarrowThreads, 0, stream, a);
 }
 
 template <typename T, typename R, int CPW, bool KEEP>
@@ -780,14 +779,13 @@ cudaError_t launch_few(const NormResidualArgs& a, cudaStream_t stream) {
     const int teams = warps == 1 ? 4 : 1;
     const int64_t ctas = (a.rows + teams - 1) / teams;
     const dim3 block(32 * warps, teams);
-    if (a.vec) norm_rows_kernel<T, R, CPW, KEEP, true><<<uint32_t(ctas), block, 0, stream>>>(a);
-    else norm_rows_kernel<T, R, CPW, KEEP, false><<<uint32_t(ctas), block, 0, stream>>>(a);
-    return cudaGetLastError();
+    if (a.vec) return launch_on(norm_rows_kernel<T, R, CPW, KEEP, true>, uint32_t(ctas), block, 0, stream, a);
+    return launch_on(norm_rows_kernel<T, R, CPW, KEEP, false>, uint32_t(ctas), block, 0, stream, a);
 }
 
 // The streaming kernel for rows of CPW chunks a warp; false: not for this call.
 template <typename T, typename R, int CPW>
-bool launch_stream(const NormResidualArgs& a, int num_sms, cudaStream_t stream) {
+bool launch_stream(const NormResidualArgs& a, int num_sms, cudaStream_t stream, cudaError_t& e) {
     using Row = StreamRow<T, R, CPW>;
     const int warps = (a.dim + int(Row::COLS) - 1) / int(Row::COLS);
     int vectors = 0;
@@ -805,8 +803,8 @@ bool launch_stream(const NormResidualArgs& a, int num_sms, cudaStream_t stream) 
     if (teams * warps < 10 && vectors <= 2) return false;
     const dim3 block(32 * warps, teams);
     const uint32_t smem = uint32_t(vector_bytes + teams * team_bytes);
-    if (a.vec) norm_stream_kernel<T, R, CPW, true><<<num_sms, block, smem, stream>>>(a);
-    else norm_stream_kernel<T, R, CPW, false><<<num_sms, block, smem, stream>>>(a);
+    e = a.vec ? launch_on(norm_stream_kernel<T, R, CPW, true>, num_sms, block, smem, stream, a)
+              : launch_on(norm_stream_kernel<T, R, CPW, false>, num_sms, block, smem, stream, a);
     return true;
 }
 
@@ -819,10 +817,11 @@ cudaError_t launch_types(const NormResidualArgs& a, int num_sms, cudaStream_t st
     // 55 us; with fewer rows one warp a row of the other kernel is as good (1000 x
     // 256 2.8 and 2.7 us).
     if (a.dim <= kChunk && a.rows >= 8 * num_sms) return launch_narrow<T, R, 32>(a, num_sms, stream);
+    cudaError_t e = cudaSuccess;
     const bool streamed = a.dim <= kChunk       ? false
-                          : a.dim <= 2 * kChunk ? launch_stream<T, R, 2>(a, num_sms, stream)
-                                                : launch_stream<T, R, 4>(a, num_sms, stream);
-    if (streamed) return cudaGetLastError();
+                          : a.dim <= 2 * kChunk ? launch_stream<T, R, 2>(a, num_sms, stream, e)
+                                                : launch_stream<T, R, 4>(a, num_sms, stream, e);
+    if (streamed) return e;
     if (a.dim <= kMaxWarps * kChunk) return launch_few<T, R, 1, true>(a, stream);
     if (a.dim <= 2 * kMaxWarps * kChunk) return launch_few<T, R, 1, false>(a, stream);
     return launch_few<T, R, 2, false>(a, stream);

@@ -842,8 +842,7 @@ cudaError_t launch_pair(const GemmFp8Args& a, int num_sms, cudaStream_t stream) 
     const int64_t tiles = (int64_t(a.M) + 2 * kTileM - 1) / (2 * kTileM) * ((int64_t(a.N) + Cfg::BN - 1) / Cfg::BN);
     if (tiles > (1 << 30)) return cudaErrorInvalidValue;
     const int pairs = int(tiles < num_sms / 2 ? tiles : num_sms / 2);
-    gemm_fp8_pair_kernel<OUT><<<2 * pairs, Cfg::THREADS, Cfg::SMEM, stream>>>(tx, tw, ty, a);
-    return cudaGetLastError();
+    return launch_on(gemm_fp8_pair_kernel<OUT>, 2 * pairs, Cfg::THREADS, Cfg::SMEM, stream, tx, tw, ty, a);
 }
 
 // Up to 32 rows the narrow tiles.  Above, what takes less by the two kernels'

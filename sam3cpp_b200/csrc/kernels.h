@@ -96,6 +96,18 @@ cudaError_t launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t 
     return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
+// A plain launch that answers with its own status: cudaGetLastError after
+// <<<>>> would answer with (and clear) an older error of the caller's.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_on(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
 // C[M,N] = A[M,K] * B[N,K]^T with A, B fp16 row-major (K contiguous).
 // Requires K % 64 == 0 and N % 32 == 0; A and B 16-byte aligned rows.
 cudaError_t launch_gemm(const __half* A, const __half* B, const GemmArgs& args, int epi, int num_sms,

@@ -56,10 +56,10 @@ int run_on(const char* op, int device, Launch launch) {
     DeviceView dev;
     if (device_view(device, &dev)) return -1;
     const DeviceScope scope(device);
-    if (scope.error != cudaSuccess) return refuse(op, cudaGetErrorString(scope.error));
-    const cudaError_t e = launch(dev);
-    if (e != cudaSuccess) return refuse(op, cudaGetErrorString(e));
-    return 0;
+    const cudaError_t e = scope.error != cudaSuccess ? scope.error : launch(dev);
+    if (e == cudaSuccess) return 0;
+    cudaGetLastError();   // reported here: the caller's next check must not find it again
+    return refuse(op, cudaGetErrorString(e));
 }
 
 #define S3T_CATCH(op)                                                    \

@@ -284,10 +284,8 @@ cudaError_t launch(const QuantizeArgs& a, cudaStream_t stream) {
     const int64_t rb = (a.rows + (blocks ? kScaleBlock : kRowsPerCta<T>) - 1) / (blocks ? kScaleBlock : kRowsPerCta<T>);
     if (rb > 0x7fffffff / cb) return cudaErrorInvalidValue;
     if (blocks)
-        quantize_blocks_kernel<T, VEC><<<uint32_t(rb * cb), kBlockThreads<T>, 0, stream>>>(a, uint32_t(cb));
-    else
-        quantize_rows_kernel<T, VEC><<<uint32_t(rb * cb), kThreads, 0, stream>>>(a, uint32_t(cb));
-    return cudaGetLastError();
+        return launch_on(quantize_blocks_kernel<T, VEC>, uint32_t(rb * cb), kBlockThreads<T>, 0, stream, a, uint32_t(cb));
+    return launch_on(quantize_rows_kernel<T, VEC>, uint32_t(rb * cb), kThreads, 0, stream, a, uint32_t(cb));
 }
 
 }  // namespace

@@ -223,8 +223,7 @@ cudaError_t launch(const RotaryArgs& a, cudaStream_t stream) {
             lanes = l;
         }
     }
-    rotary_kernel<T, V, INTERLEAVED><<<uint32_t(ctas), kThreads, 0, stream>>>(a, int(tpc), turned, slots, lanes);
-    return cudaGetLastError();
+    return launch_on(rotary_kernel<T, V, INTERLEAVED>, uint32_t(ctas), kThreads, 0, stream, a, int(tpc), turned, slots, lanes);
 }
 
 template <typename T, bool INTERLEAVED>

@@ -44,10 +44,15 @@ int fail(const std::string& msg) {
     return -1;
 }
 
+// An error that is reported is cleared too: the caller's next check of the
+// runtime's last error must not find it again.
 #define S3T_CUDA(call)                                                                    \
     do {                                                                                  \
         cudaError_t _e = (call);                                                          \
-        if (_e != cudaSuccess) return fail(std::string(#call) + ": " + cudaGetErrorString(_e)); \
+        if (_e != cudaSuccess) {                                                          \
+            cudaGetLastError();                                                           \
+            return fail(std::string(#call) + ": " + cudaGetErrorString(_e));              \
+        }                                                                                 \
     } while (0)
 
 const char* kPrefix = "backbone.vision_backbone.trunk";
@@ -873,7 +878,10 @@ int s3t::set_last_error(const char* msg) { return fail(msg); }
 int s3t::device_view(int device, DeviceView* out) {
     // device_state leaves the device it prepares current; the caller's comes back.
     const DeviceScope scope(device);
-    if (scope.error != cudaSuccess) return fail(std::string("cudaSetDevice: ") + cudaGetErrorString(scope.error));
+    if (scope.error != cudaSuccess) {
+        cudaGetLastError();
+        return fail(std::string("cudaSetDevice: ") + cudaGetErrorString(scope.error));
+    }
     DeviceState* ds = nullptr;
     if (device_state(device, &ds)) return -1;
     out->num_sms = ds->num_sms;

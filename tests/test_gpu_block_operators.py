@@ -706,6 +706,51 @@ def test_calls_from_two_threads(torch):
         assert all(torch.equal(a, b) for a, b in zip(alone[seed], together[seed]))
 
 
+def test_errors_stay_with_their_callers(torch):
+    """A refused device leaves no error in the runtime for the next check of the caller's (torch makes one after every
+    launch), and a call does not report an error that was there before it."""
+    import ctypes
+    runtime = ctypes.CDLL("libcudart.so.12")
+    x, w = Eight(torch, 4, 256), Eight(torch, 256, 256, 128)
+    for t in (x, w):
+        t.q[:] = 0
+        t.scale[:] = 1
+    v, y = torch.ones(4, 256, device="cuda"), torch.zeros(4, 256, device="cuda")
+    wide, wide_y = torch.ones(2, 8192, device="cuda"), torch.zeros(2, 8192, device="cuda")
+    many, many_y = torch.ones(5000, 512, device="cuda"), torch.zeros(5000, 512, device="cuda")
+    many8, many8_y = Eight(torch, 2600, 256), torch.zeros(2600, 256, device="cuda")
+    freq, positions = torch.ones(32, device="cuda", dtype=torch.float64), torch.zeros(4, device="cuda", dtype=torch.int64)
+    view = s3t.RotaryView(v.data_ptr(), y.data_ptr(), 4, 256, 64, 256, 64)
+
+    def norm(device, rows, dim, x, u):
+        s3t.norm_residual(device, s3t.NormArgs(rows=rows, dim=dim, eps=1e-5, resid_scale=1.0, x=x.data_ptr(), x_stride=dim,
+                                               u=s3t.Matrix(u.data_ptr(), dim)))
+
+    calls = [
+        lambda d: s3t.quantize_fp8(d, s3t.TYPE_F32, v.data_ptr(), 4, 256, 256, 1, x.matrix),
+        lambda d: s3t.quantize_fp8(d, s3t.TYPE_F32, v.data_ptr(), 4, 256, 256, 128, w.matrix),
+        lambda d: s3t.gemm_fp8(d, x.matrix, w.matrix, None, 4, 256, 256, 0, s3t.TYPE_F32, s3t.Matrix(y.data_ptr(), 256)),
+        lambda d: s3t.gemm_fp8(d, many8.matrix, w.matrix, None, 2600, 256, 256, 0, s3t.TYPE_F32,
+                               s3t.Matrix(many8_y.data_ptr(), 256)),
+        lambda d: norm(d, 4, 256, v, y),
+        lambda d: norm(d, 16, 64, v, y),
+        lambda d: norm(d, 2, 8192, wide, wide_y),
+        lambda d: norm(d, 5000, 512, many, many_y),
+        lambda d: s3t.rotary(d, freq.data_ptr(), 64, 1.0, positions.data_ptr(), 4, s3t.TYPE_F32, 64, view),
+    ]
+    torch.cuda.synchronize()
+    for call in calls:
+        assert runtime.cudaPeekAtLastError() == 0
+        with pytest.raises(s3t.S3TError):
+            call(4096)
+        assert runtime.cudaPeekAtLastError() == 0
+        error = runtime.cudaSetDevice(4096)             # the caller's own, on the host only
+        assert error != 0 and runtime.cudaPeekAtLastError() == error
+        call(0)
+        assert runtime.cudaGetLastError() == error
+    torch.cuda.synchronize()
+
+
 def test_small_operators_in_a_graph(torch):
     """Quantization, the norms and rotary captured once and replayed on new values in the same buffers."""
     rows, dim = 9, 256
