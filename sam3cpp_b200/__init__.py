@@ -40,6 +40,26 @@ class S3TError(RuntimeError):
     pass
 
 
+def _fits(bits: int, *values: int) -> None:
+    """Refuses what ctypes would wrap to another number of `bits` bits.  The calls below come here only where one of
+    their numbers is negative or too large: a shift of their union says so, which costs 0.1 us of a call's 10."""
+    for v in values:
+        if not -1 << (bits - 1) <= v < 1 << (bits - 1):
+            raise S3TError(f"{v} does not fit an argument of {bits} bits")
+
+
+def _refuse_wrapping(structure: type, name: str) -> None:
+    """Makes a 32-bit size of a C structure refuse what does not fit."""
+    raw = getattr(structure, name)
+    put_raw = raw.__set__
+
+    def put(self, v):
+        if v >> 31:
+            _fits(32, v)
+        put_raw(self, v)
+    setattr(structure, name, property(raw.__get__, put))
+
+
 class Matrix(C.Structure):
     """s3t_matrix: rows in device memory, `stride` elements apart, and for 8-bit matrices the scale of
     column group g of row block i at scale[g * scale_stride + i]."""
@@ -60,6 +80,10 @@ class RotaryView(C.Structure):
     """s3t_rotary_view: the heads of one tensor, read at x and written at out (which may be x)."""
     _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("heads", C.c_int32), ("x_token_stride", C.c_int64),
                 ("x_head_stride", C.c_int64), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64)]
+
+
+_refuse_wrapping(NormArgs, "dim")
+_refuse_wrapping(RotaryView, "heads")
 
 
 _lib = None
@@ -383,6 +407,9 @@ def quantize_fp8(device: int, type: int, x_ptr: int, rows: int, cols: int, x_str
                  stream: int = 0) -> None:
     """Device rows of `type` (TYPE_F32, TYPE_F16 or TYPE_BF16) -> the e4m3 matrix `q` with a scale per 128 columns
     and `block_rows` rows (1: an activation, 128: a weight): s3t_quantize_fp8."""
+    if (type | block_rows) >> 31 or (rows | cols) >> 63:
+        _fits(32, type, block_rows)
+        _fits(64, rows, cols)
     check(lib().s3t_quantize_fp8(device, type, x_ptr, rows, cols, x_stride, block_rows, q, stream))
 
 
@@ -390,6 +417,8 @@ def gemm_fp8(device: int, x: Matrix, w: Matrix, bias_ptr: int | None, m: int, n:
              y: Matrix, stream: int = 0) -> None:
     """y [m][n] = act(x [m][k] w [n][k]^T + bias) of e4m3 matrices with block scales (x per row, w per 128 rows);
     act 1 is GELU; y_type TYPE_F32, TYPE_F16, TYPE_BF16, or TYPE_E4M3 for the next product's x: s3t_gemm_fp8."""
+    if (m | n | k | act | y_type) >> 31:
+        _fits(32, m, n, k, act, y_type)
     check(lib().s3t_gemm_fp8(device, x, w, bias_ptr, m, n, k, act, y_type, y, stream))
 
 
@@ -403,7 +432,8 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: int = ROTAR
                        original_len: float = 0.0, fast: float = 32.0, slow: float = 1.0) -> tuple[np.ndarray, float]:
     """(radians per position of each pair as float64, magnitude) of rotary positions, scaled for a context `factor`
     times `original_len`: s3t_rotary_frequencies.  Host only."""
-    freq = np.empty(max(rot_dim // 2, 1), np.float64)
+    _fits(32, rot_dim)
+    freq = np.empty(min(max(rot_dim // 2, 1), 512), np.float64)     # larger ones are refused
     magnitude = C.c_float()
     check(lib().s3t_rotary_frequencies(rot_dim, base, scaling, factor, original_len, fast, slow,
                                        freq.ctypes.data_as(C.POINTER(C.c_double)), C.byref(magnitude)))
@@ -414,5 +444,8 @@ def rotary(device: int, freq_ptr: int, rot_dim: int, magnitude: float, positions
            head_dim: int, q: RotaryView, k: RotaryView | None = None, flags: int = 0, stream: int = 0) -> None:
     """Turns the first rot_dim columns of the heads of q and k by position times frequency (device float64
     frequencies, int64 positions; a negative position leaves its token unwritten): s3t_rotary."""
+    if (rot_dim | head_dim) >> 31 or tokens >> 63:
+        _fits(32, rot_dim, head_dim)
+        _fits(64, tokens)
     check(lib().s3t_rotary(device, freq_ptr, rot_dim, magnitude, positions_ptr, tokens, type, head_dim, q, k, flags,
                            stream))

@@ -184,6 +184,40 @@ def test_empty_calls_take_the_null_pointers_of_empty_tensors():
         s3t.rotary(0, A, 31, 1.0, None, 0, s3t.TYPE_F16, 64, v)
 
 
+WRAP = 1 << 32       # taken modulo 2^32 each of these sizes would be an empty or a valid call
+
+
+@pytest.mark.parametrize("call", [
+    lambda: s3t.quantize_fp8(0, s3t.TYPE_F32, A, 0, 200, 200, WRAP + 1, eight()),
+    lambda: s3t.quantize_fp8(0, WRAP, A, 0, 200, 200, 1, eight()),
+    lambda: s3t.quantize_fp8(0, s3t.TYPE_F32, A, 1 << 64, 200, 200, 1, eight()),
+    lambda: s3t.gemm_fp8(0, eight(), eight(), None, WRAP, 200, 200, 0, s3t.TYPE_F16, s3t.Matrix(A, 200)),
+    lambda: s3t.gemm_fp8(0, eight(), eight(), None, 5, -WRAP, 200, 0, s3t.TYPE_F16, s3t.Matrix(A, 200)),
+    lambda: s3t.gemm_fp8(0, eight(), eight(), None, 0, 200, WRAP + 200, 0, s3t.TYPE_F16, s3t.Matrix(A, 200)),
+    lambda: s3t.norm_residual(0, s3t.NormArgs(**{**NORM, "rows": 0, "dim": WRAP + 200})),
+    lambda: s3t.norm_residual(0, s3t.NormArgs(0, WRAP + 200)),
+    lambda: s3t.rotary(0, A, WRAP + 32, 1.0, A, 0, s3t.TYPE_F16, 64, ROTARY["q"]),
+    lambda: s3t.rotary(0, A, 32, 1.0, A, 0, s3t.TYPE_F16, WRAP + 64, ROTARY["q"]),
+    lambda: s3t.rotary(0, A, 32, 1.0, A, 1 << 64, s3t.TYPE_F16, 64, ROTARY["q"]),
+    lambda: s3t.rotary(0, A, 32, 1.0, A, 0, s3t.TYPE_F16, 64, s3t.RotaryView(A, A, WRAP + 4, 256, 64, 256, 64)),
+    lambda: s3t.rotary_frequencies(WRAP + 64),
+])
+def test_sizes_do_not_wrap(call):
+    with refused("does not fit"):
+        call()
+
+
+def test_structure_fields_hold_what_they_are_given():
+    a = s3t.NormArgs(7, 1024, s3t.TYPE_BF16, u_type=s3t.TYPE_E4M3, eps=0.5)
+    assert (a.rows, a.dim, a.type, a.resid_type, a.u_type, a.eps) == (7, 1024, s3t.TYPE_BF16, 0, s3t.TYPE_E4M3, 0.5)
+    a.dim = 1 << 20
+    assert a.dim == 1 << 20
+    with refused("does not fit"):
+        a.dim = -(1 << 31) - 1
+    assert a.dim == 1 << 20
+    assert s3t.RotaryView(heads=4).heads == 4
+
+
 def test_a_call_without_a_gpu_is_an_error():
     import torch
     if torch.cuda.is_available():
