@@ -301,7 +301,7 @@ int s3t_quantize_fp8(int device, int type, const void *x_dev, int64_t rows, int6
  * F32, F16, BF16, or E4M3, which holds what s3t_quantize_fp8 with block_rows 1
  * makes of the F32 result (y->scale for [ceil(N / 128)][scale_stride >= M]),
  * ready to be the next product's x.  Any M, N >= 0
- * and K >= 1, up to 2^30 each.  The result does not depend on what else runs.  A wait that runs
+ * and K >= 1 (without rows or columns of y K >= 0), up to 2^30 each.  The result does not depend on what else runs.  A wait that runs
  * out inside the kernel is reported by s3t_device_status. */
 int s3t_gemm_fp8(int device, const s3t_matrix *x, const s3t_matrix *w, const float *bias_dev, int M, int N, int K,
                  int act, int y_type, const s3t_matrix *y, void *stream);

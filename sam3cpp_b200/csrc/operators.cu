@@ -108,10 +108,11 @@ int s3t_gemm_fp8(int device, const s3t_matrix* x, const s3t_matrix* w, const flo
         const char* op = "gemm_fp8";
         const int kind = element_kind(y_type);
         if (kind < 0) return refuse(op, "y must be F32, F16, BF16 or E4M3");
-        if (M < 0 || N < 0 || K < 1) return refuse(op, "needs M >= 0, N >= 0 and K >= 1");
+        const bool empty = M == 0 || N == 0;   // then there may be no K either
+        if (M < 0 || N < 0 || K < (empty ? 0 : 1)) return refuse(op, "needs M >= 0, N >= 0 and K >= 1");
         if (M > kMost || N > kMost || K > kMost) return refuse(op, "M, N and K must be at most 2^30");
         if (act != 0 && act != 1) return refuse(op, "act must be 0 (none) or 1 (GELU)");
-        if (M == 0 || N == 0) return 0;
+        if (empty) return 0;
         if (const char* why = bad_eight(x, K, M)) return refuse(op, std::string("x: ") + why);
         if (const char* why = bad_eight(w, K, blocks(N))) return refuse(op, std::string("w: ") + why);
         if (!aligned(bias, 4)) return refuse(op, "bias must be 4-byte aligned");

@@ -184,6 +184,15 @@ def test_empty_calls_take_the_null_pointers_of_empty_tensors():
         s3t.rotary(0, A, 31, 1.0, None, 0, s3t.TYPE_F16, 64, v)
 
 
+@pytest.mark.parametrize("y_type", [s3t.TYPE_F16, s3t.TYPE_E4M3])
+def test_empty_products_need_no_columns(y_type):
+    none = s3t.Matrix(None, 0, None, 0)
+    for m, n in ((0, 200), (5, 0), (0, 0)):
+        s3t.gemm_fp8(0, none, none, None, m, n, 0, 0, y_type, none)
+        with refused("K >= 1"):
+            s3t.gemm_fp8(0, none, none, None, m, n, -1, 0, y_type, none)
+
+
 WRAP = 1 << 32       # taken modulo 2^32 each of these sizes would be an empty or a valid call
 
 
