@@ -366,7 +366,9 @@ int s3t_rotary_frequencies(int rot_dim, double base, int scaling, double factor,
 /* The heads of one tensor: token t, head h, column c is
  * x[t * x_token_stride + h * x_head_stride + c], so token-major, head-major
  * and packed projections (a pointer to the first head) are all views.  out may
- * be x itself, with the same strides. */
+ * be x itself, with the same strides.  Heads of x may overlap (a stride of 0
+ * turns one head by every position); heads of out must not, neither with one
+ * another nor with the other tensor's. */
 typedef struct s3t_rotary_view {
     const void *x;
     void *out;

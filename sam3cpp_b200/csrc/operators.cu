@@ -51,6 +51,19 @@ const char* bad_eight(const s3t_matrix* m, int64_t cols, int64_t scales) {
     return nullptr;
 }
 
+// Whether two of tokens x heads runs of `dim` elements, at t * token + h * head,
+// share an element.  Strides are at least dim where there are two to a stride.
+bool runs_overlap(int64_t tokens, int64_t token, int heads, int64_t head, int dim) {
+    using Wide = __int128;
+    if (tokens == 1 || heads == 1) return false;
+    if (token >= Wide(heads - 1) * head + dim || head >= Wide(tokens - 1) * token + dim) return false;   // token- or head-major
+    for (int h = 1; h < heads; ++h) {   // the tokens next to a head of token 0
+        const Wide at = Wide(h) * head, t = at / token, past = at - t * token;
+        if ((t < tokens && past < dim) || (t + 1 < tokens && token - past < dim)) return true;
+    }
+    return false;
+}
+
 template <typename Launch>
 int run_on(const char* op, int device, Launch launch) {
     DeviceView dev;
@@ -281,6 +294,8 @@ int s3t_rotary(int device, const double* freq, int rot_dim, float magnitude, con
                 return refuse(op, "the strides of out must be at least head_dim");
             if (s->x == s->out && (s->x_token_stride != s->out_token_stride || s->x_head_stride != s->out_head_stride))
                 return refuse(op, "in place needs the same strides of x and out");
+            if (runs_overlap(tokens, s->out_token_stride, s->heads, s->out_head_stride, head_dim))
+                return refuse(op, "heads of out overlap");
             RotaryPart& p = a.part[i];
             p.x = s->x;
             p.out = s->out;
@@ -292,6 +307,8 @@ int s3t_rotary(int device, const double* freq, int rot_dim, float magnitude, con
             marks |= (reinterpret_cast<uintptr_t>(s->x) | reinterpret_cast<uintptr_t>(s->out)) / uintptr_t(eb);
             marks |= uint64_t(p.x_token) | uint64_t(p.x_head) | uint64_t(p.out_token) | uint64_t(p.out_head);
         }
+        if (k && (q->out == k->out || q->out == k->x || k->out == q->x))
+            return refuse(op, "q and k must not be written over one another");
         a.run = marks % uint64_t(16 / eb) == 0 ? 16 / eb : marks % 2 == 0 ? 2 : 1;
         a.freq = freq;
         a.rot = rot_dim;

@@ -143,6 +143,14 @@ ROTARY = dict(freq=A, rot=32, positions=A, tokens=5, type=s3t.TYPE_F16, dim=64,
     (dict(q=s3t.RotaryView(A, A + 16, 4, -256, 64, 256, 64)), "negative"),
     (dict(q=s3t.RotaryView(A, A + 16, 4, 256, 64, 256, 32)), "at least head_dim"),
     (dict(k=s3t.RotaryView(A, A, 4, 256, 64, 512, 64)), "in place"),
+    (dict(q=s3t.RotaryView(A, A + 16, 4, 256, 64, 64, 64)), "overlap"),           # token t, head h where t + 1, h - 1 is
+    (dict(q=s3t.RotaryView(A, A + 16, 4, 256, 64, 64, 128)), "overlap"),
+    (dict(q=s3t.RotaryView(A, A + 16, 4, 256, 64, 192, 256)), "overlap"),         # token 4, head 0 on token 0, head 3
+    (dict(q=s3t.RotaryView(A, A + 16, 2, 256, 64, 1 << 62, (1 << 62) + 63)), "overlap"),
+    (dict(q=s3t.RotaryView(A, A + 16, 2, 256, 64, (1 << 61) + 63, 1 << 61)), "overlap"),
+    (dict(k=s3t.RotaryView(A + 4096, A, 4, 256, 64, 256, 64)), "over one another"),
+    (dict(q=s3t.RotaryView(A, A + 4096, 4, 256, 64, 256, 64), k=s3t.RotaryView(A + 4096, A + 8192, 4, 256, 64, 256, 64)),
+     "over one another"),
 ])
 def test_rotary_refusals(change, match):
     a = {**ROTARY, **change}

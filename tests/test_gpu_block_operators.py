@@ -625,6 +625,25 @@ def test_rotary_against_64_bits(torch, kind, interleaved, tokens, heads, kheads,
         assert torch.equal(got[there][..., rot:], x[:, : heads * dim].view(tokens, heads, dim)[there][..., rot:])
 
 
+@pytest.mark.parametrize("tokens, heads, token, head", [(5, 3, 192, 256), (9, 2, 160, 640 + 80), (1, 4, 0, 64), (6, 1, 64, 0)])
+def test_rotary_layouts_that_interleave(torch, tokens, heads, token, head):
+    """Heads of out between one another's tokens, neither token- nor head-major, and strides that nothing uses; every
+    head of x the same one (strides of 0)."""
+    dim = 64
+    x = torch.randn(dim, device="cuda")
+    freq, _ = s3t.rotary_frequencies(dim)
+    freq, positions = torch.from_numpy(freq).cuda(), torch.arange(tokens, device="cuda") * 17
+    at = torch.arange(tokens)[:, None] * token + torch.arange(heads) * head
+    out = torch.full((int(at.max()) + dim + 8,), 5.0, device="cuda")
+    s3t.rotary(0, freq.data_ptr(), dim, 1.0, positions.data_ptr(), tokens, s3t.TYPE_F32, dim,
+               s3t.RotaryView(x.data_ptr(), out.data_ptr(), heads, 0, 0, token, head))
+    want, e = turned64(torch, x.double().expand(tokens, heads, dim), positions, freq, dim, 1.0, False, False)
+    places = (at[..., None] + torch.arange(dim)).cuda()
+    assert ((out[places].double() - want).abs() <= e + want.abs() * U).all()
+    out[places] = 5.0
+    assert (out == 5.0).all()
+
+
 def test_rotary_offsets_past_32_bits(torch):
     """Token strides that put the last token over 2^32 elements away (a slot of a long cache)."""
     stride, tokens, dim = (1 << 31) + 64, 3, 64
