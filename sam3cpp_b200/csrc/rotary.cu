@@ -4,9 +4,12 @@
 // where a pair is columns (2i, 2i + 1) (interleaved) or (i, i + rot / 2)
 // (halves); the other columns pass through.
 //
-// The angle is taken in 64 bits as turns, position * frequency / 2 pi, and only
-// its fraction goes to 32 bits: at position 10^6 an fp32 angle is off by up to
-// 0.03 rad, this one by 2^-25 turns.  A CTA takes the tokens' cosines and sines
+// The angle is taken in 64 bits as turns, position * frequency / 2 pi, and its
+// fraction goes to 32 bits in two parts: at position 10^6 an fp32 angle is off
+// by up to 0.03 rad, this one's cosine and sine by two of their own roundings.
+// (One part alone was off by 2^-27 turns: a third more error of fp32 heads, rms;
+// the second costs nothing where heads are many, 17.3 -> 18.6 us for 65536
+// tokens of one head of 128.)  A CTA takes the tokens' cosines and sines
 // into shared memory once for all their heads, so the trigonometry is rot / 2
 // evaluations a token and the rest is a stream over the heads: bound by HBM,
 // one read and one write of every element.
@@ -150,8 +153,11 @@ __global__ void __launch_bounds__(kThreads, INTERLEAVED ? 8 : 6)
         const int64_t pos = a.positions[t0 + t];
         double turns = double(pos) * a.freq[p] * 0.15915494309189533577;   // 1 / (2 pi)
         turns -= rint(turns);
-        float s, c;
-        sincospif(2.f * float(turns), &s, &c);
+        // What the fraction loses in 32 bits turns the pair a little further.
+        const float near = float(turns), rest = float(turns - double(near)) * 6.283185307f;
+        float s0, c0;
+        sincospif(2.f * near, &s0, &c0);
+        const float s = fmaf(c0, rest, s0), c = fmaf(-s0, rest, c0);
         table[i] = make_float2(c * a.magnitude, (a.inverse ? -s : s) * a.magnitude);
     }
     if (threadIdx.x < tokens) position[threadIdx.x] = a.positions[t0 + threadIdx.x];

@@ -625,6 +625,32 @@ def test_rotary_against_64_bits(torch, kind, interleaved, tokens, heads, kheads,
         assert torch.equal(got[there][..., rot:], x[:, : heads * dim].view(tokens, heads, dim)[there][..., rot:])
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("quarter", [0, 1, 2, 3])
+def test_rotary_next_to_quarter_turns(torch, interleaved, quarter):
+    """Heads of pairs (1, 0) answer with the cosine and sine themselves.  Next to a quarter turn one of them is small and
+    as exact as its type: sincospif to a step (2^-23), one sum's rounding (2^-24), and 1e-13 for the 64-bit angle."""
+    n, tokens = 256, 5
+    away = torch.exp(torch.linspace(math.log(1e-5), math.log(1e-2), n, dtype=torch.float64)) * (-1) ** torch.arange(n)
+    freq = (2 * math.pi * (quarter / 4 + 1 + away)).cuda()
+    positions = torch.tensor([1, 5, -1, 9, 13], device="cuda")       # whole quarter turns away from one another
+    x = torch.zeros(tokens, 2 * n, device="cuda")
+    if interleaved:
+        x[:, ::2] = 1
+    else:
+        x[:, :n] = 1
+    y = torch.full_like(x, 5.0)
+    s3t.rotary(0, freq.data_ptr(), 2 * n, 1.0, positions.data_ptr(), tokens, s3t.TYPE_F32, 2 * n,
+               s3t.RotaryView(x.data_ptr(), y.data_ptr(), 1, 2 * n, 2 * n, 2 * n, 2 * n), None,
+               s3t.ROTARY_INTERLEAVED if interleaved else 0)
+    got = y.view(tokens, n, 2) if interleaved else y.view(tokens, 2, n).transpose(1, 2)
+    angle = positions.double()[:, None] * freq
+    want = torch.stack((angle.cos(), angle.sin()), -1)
+    there = positions >= 0
+    assert ((got.double() - want).abs() <= want.abs() * (2.0 ** -23 + 2.0 ** -24) * 1.01 + 1e-13)[there].all()
+    assert (got[~there] == 5).all()
+
+
 @pytest.mark.parametrize("tokens, heads, token, head", [(5, 3, 192, 256), (9, 2, 160, 640 + 80), (1, 4, 0, 64), (6, 1, 64, 0)])
 def test_rotary_layouts_that_interleave(torch, tokens, heads, token, head):
     """Heads of out between one another's tokens, neither token- nor head-major, and strides that nothing uses; every
