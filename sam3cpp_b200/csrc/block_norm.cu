@@ -783,6 +783,27 @@ cudaError_t launch_few(const NormResidualArgs& a, cudaStream_t stream) {
     return launch_on(norm_rows_kernel<T, R, CPW, KEEP, false>, uint32_t(ctas), block, 0, stream, a);
 }
 
+// Rows a team from which the streaming kernel's set-up (the vectors' way into
+// shared memory, 20 to 50 us for wide rows) is paid for.  Up to 4096 columns
+// the other kernel keeps the vectors in registers and two rows do.  Above, it
+// reads them again for every row, so two or three teams an SM win soon, a
+// single one later, and later still with few vectors to read again or where
+// five fp32 warps are all that hide a row's latency.  Measured where the two
+// meet, post-norm and pre-norm, streamed / not, us:
+//   2 teams, 4 vectors   f32 6144     at 2 rows 31 / 29, at 3 36 / 42
+//   2 teams, 2 vectors   f32 8192     at 4 52 / 49, at 6 66 / 70; fp16 8192 at 3 38 / 33, at 6 48 / 60
+//   1 team, 4 vectors    f32 7070     at 8 68 / 63, at 12 84 / 91; fp16 9024 at 8 65 / 60, at 12 79 / 87
+//   1 team, 2 vectors    f32 9024     at 24 131 / 121, at 48 212 / 228
+//                        fp16 10240   at 16 91 / 83, at 24 112 / 122; bf16 16384 at 12 92 / 91, at 16 106 / 119
+//   5 warps of fp32      1 team, 4 vectors 5120 at 32 131 / 121, at 64 224 / 232; 3 teams, 2 vectors at 16
+//                        117 / 114, at 32 212 / 219
+template <typename T>
+int stream_rounds(int teams, int warps, int vectors, int dim) {
+    if (dim <= kMaxWarps * kChunk) return 2;
+    const int rounds = teams > 1 ? (vectors > 2 ? 3 : 6) : vectors > 2 ? 10 : sizeof(T) == 4 ? 30 : 16;
+    return sizeof(T) == 4 && warps <= 5 ? 4 * rounds : rounds;
+}
+
 // The streaming kernel for rows of CPW chunks a warp; false: not for this call.
 template <typename T, typename R, int CPW>
 bool launch_stream(const NormResidualArgs& a, int num_sms, cudaStream_t stream, cudaError_t& e) {
@@ -793,14 +814,7 @@ bool launch_stream(const NormResidualArgs& a, int num_sms, cudaStream_t stream, 
     const int vector_bytes = vectors * warps * int(Row::COLS) * 4, team_bytes = warps * kSlots * int(row_bytes<Row>(a));
     int teams = vector_bytes < kStreamBytes ? (kStreamBytes - vector_bytes) / team_bytes : 0;
     if (teams > kStreamWarps / warps) teams = kStreamWarps / warps;
-    // Two rows a team and more: the rows ahead pay for the set-up.
-    if (teams == 0 || a.rows < int64_t(2) * num_sms * teams) return false;
-    // Fewer than ten warps an SM hide too little, unless the call has more vectors
-    // than the other kernel had better read again for every row (streamed / not:
-    // 719 x 7070 fp32, 7 warps, 77 / 35 us; 2290 x 9024 fp16, 9 warps, 91 / 85
-    // us; 2290 x 8192 fp16 with four vectors, 8 warps, 85 / 114 us; 5000 x 5120
-    // bf16, 15 warps, 54 / 69 us; 5000 x 16384 fp16, 16 warps, 169 / 238 us).
-    if (teams * warps < 10 && vectors <= 2) return false;
+    if (teams == 0 || a.rows < int64_t(stream_rounds<T>(teams, warps, vectors, a.dim)) * num_sms * teams) return false;
     const dim3 block(32 * warps, teams);
     const uint32_t smem = uint32_t(vector_bytes + teams * team_bytes);
     e = a.vec ? launch_on(norm_stream_kernel<T, R, CPW, true>, num_sms, block, smem, stream, a)

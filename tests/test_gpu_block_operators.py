@@ -537,6 +537,21 @@ def test_norm_wide_rows(torch, kind, resid, rows, dim, pad):
     run_norm(torch, 20, rows, dim, kind, resid, post=False, weights=False, gate="plain", write_u=False, pad=pad)
 
 
+@pytest.mark.parametrize("kind, resid", TYPE_PAIRS)
+@pytest.mark.parametrize("rows, dim, pad", [(900, 6144, 0), (1790, 8192, 0), (1490, 9024, 0), (1481, 7070, 3), (4450, 5111, 0)])
+def test_norm_streams_of_wide_rows(torch, kind, resid, rows, dim, pad):
+    """Rows enough for teams of 5 to 9 warps, one to three an SM, to stream rows of more than 4096 columns."""
+    run_norm(torch, 21, rows, dim, kind, resid, layer=True, gate="plain", gate_rows=500, pad=pad)
+    run_norm(torch, 22, rows, dim, kind, resid, eight=True, pad=pad, in_place=True)
+
+
+@pytest.mark.parametrize("kind, resid, rows, dim", [("f32", "f32", 4445, 9024), ("f16", "f32", 2371, 12288), ("f16", "f16", 2371, 10001),
+                                                    ("bf16", "bf16", 2370, 16384), ("bf16", "f32", 2370, 13000)])
+def test_norm_streams_of_the_widest_rows(torch, kind, resid, rows, dim):
+    """One team of 9 to 16 warps an SM."""
+    run_norm(torch, 23, rows, dim, kind, resid)
+
+
 def test_norm_parts_that_are_left_out(torch):
     for dim in (256, 515):
         run_norm(torch, 1, 9, dim, "f16", "f32", branch=False)                                  # a pre-norm alone
