@@ -569,6 +569,18 @@ def test_norm_far_from_zero(torch):
         run_norm(torch, 8, 6, dim, "f32", "f32", layer=True, shift=2000.0, post=True, channel=False)
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows, dim, pad", [(131, 7, 0), (300, 32, 0), (300, 64, 0), (300, 128, 0), (67, 65, 3), (30001, 31, 0),
+                                            (1200, 130, 0), (1200, 256, 0), (1201, 255, 1), (5000, 512, 0), (5000, 1024, 0),
+                                            (4741, 1001, 0), (2400, 2050, 1), (700, 4096, 0), (900, 6144, 0)])
+def test_norm_far_from_zero_by_the_width_of_a_row(torch, kind, rows, dim, pad):
+    """As above for every lane count of the narrow kernel, and streaming teams of one and of several warps: y and x a
+    thousand spreads from zero (16-bit values of them: the spread is their rounding's)."""
+    shift = 2000.0 if kind == "f32" else 500.0
+    run_norm(torch, 24, rows, dim, kind, kind, layer=True, shift=shift, post=True, channel=False, pad=pad)
+    run_norm(torch, 25, rows, dim, kind, "f32", layer=True, shift=shift, branch=False, pad=pad)
+
+
 def test_norm_nonfinite_rows_stay_apart(torch):
     for rows, dim in ((5, 1024), (2100, 512), (5, 301), (5000, 512), (5000, 1003)):
         x = torch.randn(rows, dim, device="cuda")
