@@ -300,9 +300,12 @@ int s3t_quantize_fp8(int device, int type, const void *x_dev, int64_t rows, int6
  * itself (below, where |GELU| < 6e-9, it falls to 0 sooner than GELU).  y_type:
  * F32, F16, BF16, or E4M3, which holds what s3t_quantize_fp8 with block_rows 1
  * makes of the F32 result (y->scale for [ceil(N / 128)][scale_stride >= M]),
- * ready to be the next product's x.  Any M, N >= 0
- * and K >= 1 (without rows or columns of y K >= 0), up to 2^30 each.  The result does not depend on what else runs.  A wait that runs
- * out inside the kernel is reported by s3t_device_status. */
+ * ready to be the next product's x.  Any M, N >= 0 and K >= 1 (without rows or
+ * columns of y K >= 0), up to 2^30 each.  The result does not depend on what
+ * else runs; the order of a row's fp32 sums does depend on M, N and K, so that
+ * with another M the same row may differ by a few of their roundings (an 8-bit
+ * result by a code at a boundary).  A wait that runs out inside the kernel is
+ * reported by s3t_device_status. */
 int s3t_gemm_fp8(int device, const s3t_matrix *x, const s3t_matrix *w, const float *bias_dev, int M, int N, int K,
                  int act, int y_type, const s3t_matrix *y, void *stream);
 
@@ -313,7 +316,10 @@ int s3t_gemm_fp8(int device, const s3t_matrix *x, const s3t_matrix *w, const flo
  * Norms are RMSNorm, v / sqrt(mean(v^2) + eps) * weight + bias, or with
  * S3T_NORM_LAYER LayerNorm, (v - mean) / sqrt(var + eps) * weight + bias.  f
  * is the identity, or a sigmoid or tanh by flag.  Everything is computed in
- * fp32; u is taken from x' before its rounding to resid_type. */
+ * fp32; u is taken from x' before its rounding to resid_type.  The order of a
+ * row's sums and products depends on the count of rows, dim and alignment, so
+ * that among other rows it may differ by a few fp32 roundings.  A wait that runs
+ * out inside the kernel is reported by s3t_device_status. */
 enum {
     S3T_NORM_LAYER = 1,
     S3T_NORM_POST = 2,
@@ -357,7 +363,9 @@ int s3t_norm_residual(int device, const s3t_norm_args *args, void *stream);
  *   BY_PARTS  pairs with more than `fast` full turns within original_len keep
  *             their frequency, pairs with fewer than `slow` get freq / factor,
  *             linear in the turns between; magnitude 0.1 ln(factor) + 1 (YaRN,
- *             Peng et al. 2023)
+ *             Peng et al. 2023, the ramp as the paper has it; programs that ramp
+ *             over the index of the pair between two rounded limits have other
+ *             frequencies there: s3t_rotary takes any that the caller computes)
  * Host only: freq is host memory, to be copied to the device once. */
 enum { S3T_ROTARY_UNSCALED = 0, S3T_ROTARY_LINEAR = 1, S3T_ROTARY_BASE = 2, S3T_ROTARY_BY_PARTS = 3 };
 int s3t_rotary_frequencies(int rot_dim, double base, int scaling, double factor, double original_len, double fast,
@@ -380,7 +388,8 @@ typedef struct s3t_rotary_view {
  * positions[t] * freq[i]: pair i is columns (i, i + rot_dim / 2), or (2 i,
  * 2 i + 1) with S3T_ROTARY_INTERLEAVED; S3T_ROTARY_INVERSE turns back (the
  * magnitude still multiplies).  The other columns are copied.  The angle is
- * exact to 2^-25 turns for positions up to 2^27.  The heads of a token whose
+ * taken in 64 bits: for positions up to 2^27 and frequencies up to 1 it is exact
+ * to 2^-27 turns, and cosine and sine to 1.5 fp32 steps besides.  The heads of a token whose
  * position is negative (padding) are not written. */
 enum { S3T_ROTARY_INTERLEAVED = 1, S3T_ROTARY_INVERSE = 2 };
 int s3t_rotary(int device, const double *freq_dev, int rot_dim, float magnitude, const int64_t *positions_dev,
