@@ -389,8 +389,8 @@ typedef struct s3t_rotary_view {
  * 2 i + 1) with S3T_ROTARY_INTERLEAVED; S3T_ROTARY_INVERSE turns back (the
  * magnitude still multiplies).  The other columns are copied.  The angle is
  * taken in 64 bits: for positions up to 2^27 and frequencies up to 1 it is exact
- * to 2^-27 turns, and cosine and sine to 1.5 fp32 steps besides.  The heads of a token whose
- * position is negative (padding) are not written. */
+ * to 2^-27 turns, and cosine and sine to 1.5 fp32 steps besides.  The heads of a
+ * token whose position is negative (padding) are not written. */
 enum { S3T_ROTARY_INTERLEAVED = 1, S3T_ROTARY_INVERSE = 2 };
 int s3t_rotary(int device, const double *freq_dev, int rot_dim, float magnitude, const int64_t *positions_dev,
                int64_t tokens, int type, int head_dim, const s3t_rotary_view *q, const s3t_rotary_view *k, int flags,

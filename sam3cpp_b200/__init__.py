@@ -42,7 +42,7 @@ class S3TError(RuntimeError):
 
 def _fits(bits: int, *values: int) -> None:
     """Refuses what ctypes would wrap to another number of `bits` bits.  The calls below come here only where one of
-    their numbers is negative or too large: a shift of their union says so, which costs 0.1 us of a call's 10."""
+    their numbers is negative or too large: a shift of their union says so, which costs 0.2 us of a call's 10."""
     for v in values:
         if not -1 << (bits - 1) <= v < 1 << (bits - 1):
             raise S3TError(f"{v} does not fit an argument of {bits} bits")

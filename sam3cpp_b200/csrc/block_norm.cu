@@ -796,12 +796,13 @@ cudaError_t launch_few(const NormResidualArgs& a, cudaStream_t stream) {
 //   1 team, 2 vectors    f32 9024     at 24 131 / 121, at 48 212 / 228
 //                        fp16 10240   at 16 91 / 83, at 24 112 / 122; bf16 16384 at 12 92 / 91, at 16 106 / 119
 //   5 warps of fp32      1 team, 4 vectors 5120 at 32 131 / 121, at 64 224 / 232; 3 teams, 2 vectors at 16
-//                        117 / 114, at 32 212 / 219
+//                        117 / 114, at 32 212 / 219; 2 teams, 4 vectors 4352 at 5 33 / 31, at 15 73 / 90
 template <typename T>
 int stream_rounds(int teams, int warps, int vectors, int dim) {
     if (dim <= kMaxWarps * kChunk) return 2;
     const int rounds = teams > 1 ? (vectors > 2 ? 3 : 6) : vectors > 2 ? 10 : sizeof(T) == 4 ? 30 : 16;
-    return sizeof(T) == 4 && warps <= 5 ? 4 * rounds : rounds;
+    if (sizeof(T) == 2 || warps > 5) return rounds;
+    return (teams > 1 && vectors > 2 ? 2 : 4) * rounds;
 }
 
 // The streaming kernel for rows of CPW chunks a warp; false: not for this call.

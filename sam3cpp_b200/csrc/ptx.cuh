@@ -604,7 +604,7 @@ S3T_DEV float max_nan(float a, float b) {
 // Two lanes of GELU with one 2^x each and no reciprocal: GELU(x) = relu(x) -
 // a Q(a), a = |x|, Q(a) = erfc(a / sqrt 2) / 2 = 2^P(a), where P is a
 // polynomial of degree 8 fitted here to log2 Q on [0, 6]: the largest error
-// relative to the smaller of 0.5 and 1000 Q is least, so it stays within
+// relative to the smaller of 0.5 and 2000 Q is least, so it stays within
 // 6.3e-8 of Q and within 2.3e-4 of Q's own value.  The second bound is for
 // results that are scaled by their block's largest: blocks of nothing but
 // GELU's tail have accurate scales too.  With the steps in fp32 and 2^x good to
